@@ -29,10 +29,12 @@ MOE_PATH_AUTO, MOE_PATH_GEMV, MOE_PATH_TENSOR, MOE_PATH_GEMV_PHASED = 0, 1, 2, 3
 MOE_PATH_GEMV_FUSED = 4
 MOE_PATH_DIGITS = 5
 MOE_QUANT_INT8, MOE_QUANT_INT4 = 0, 1
+MOE_DT_F16, MOE_DT_BF16, MOE_DT_F32 = 2, 3, 4
 
 # Every symbol the header declares, with (restype, argtypes).
 P, SZ, I32, U32, U64, F32 = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32,
                              ctypes.c_uint64, ctypes.c_float)
+I64 = ctypes.c_int64
 PP = ctypes.POINTER(ctypes.c_void_p)
 
 
@@ -41,6 +43,22 @@ class MoeDims(ctypes.Structure):
                 ("num_experts", ctypes.c_int32), ("top_k", ctypes.c_int32),
                 ("norm_topk_prob", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
                 ("num_layers", ctypes.c_int32)]
+
+
+class MoeGroupedDesc(ctypes.Structure):
+    _fields_ = [("num_experts", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("ld_x", ctypes.c_int64),
+                ("ld_w", ctypes.c_int64), ("expert_stride", ctypes.c_int64),
+                ("ld_out", ctypes.c_int64)]
+
+
+class MoeBlockNormDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("hidden", ctypes.c_int32),
+                ("res_dtype", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("ld_res", ctypes.c_int64), ("ld_block", ctypes.c_int64),
+                ("post_norm", ctypes.c_int32), ("residual_scale", ctypes.c_float),
+                ("eps", ctypes.c_float)]
 
 
 class MoeKernelTime(ctypes.Structure):
@@ -99,6 +117,19 @@ SIGNATURES = {
     "moe_set_graphs": (I32, [P, I32]),
     "moe_set_wait_limit": (I32, [P, U64]),
     "moe_debug_wait_flag": (I32, [P, P]),
+    "moe_get_stream": (P, [P]),
+    "moe_grouped_mm": (I32, [P, ctypes.POINTER(MoeGroupedDesc), P, P, P, P, P]),
+    "moe_grouped_mm_dgrad": (I32, [P, ctypes.POINTER(MoeGroupedDesc), P, P, P, P, P]),
+    "moe_grouped_mm_wgrad": (I32, [P, ctypes.POINTER(MoeGroupedDesc), P, P, P, P, P]),
+    "moe_mxfp4_code_stride": (SZ, [I32]),
+    "moe_mxfp4_scale_stride": (SZ, [I32]),
+    "moe_mxfp4_quantize": (I32, [P, P, I32, I64, I32, P, I32, I32, P, P, P]),
+    "moe_mxfp4_dequantize": (I32, [P, P, P, I32, I32, P, I32, I64, P]),
+    "moe_grouped_mm_mxfp4": (I32, [P, I32, I32, I32, I32, P, P, P, P, P, P, I32, I64, P]),
+    "moe_block_norm": (I32, [P, ctypes.POINTER(MoeBlockNormDesc), P, P, P, P, P, P, P, P]),
+    "moe_block_norm_backward_workspace": (SZ, [P, I32, I32]),
+    "moe_block_norm_backward": (I32, [P, ctypes.POINTER(MoeBlockNormDesc), P, P, P, P, P, P, P,
+                                      P, P, P, P, P, P, SZ, P]),
     "moe_debug_stream_read": (I32, [P, SZ, P, P]),
 }
 

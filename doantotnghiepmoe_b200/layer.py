@@ -13,7 +13,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import (MOE_OK, MOE_ROUTER_BF16, MOE_ROUTER_F32, MoeDims, MoeError, lib,
+from ._lib import (MOE_DT_BF16, MOE_DT_F16, MOE_DT_F32, MOE_ERR_INVALID, MOE_OK, MOE_ROUTER_BF16,
+                   MOE_ROUTER_F32, MoeBlockNormDesc, MoeDims, MoeError, MoeGroupedDesc, lib,
                    ptr_array)
 
 
@@ -30,6 +31,16 @@ class MoeConfig:
 
 def _ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def _dt(t) -> int:
+    """MOE_DT_* of a floating-point tensor."""
+    import torch
+    code = {torch.float32: MOE_DT_F32, torch.float16: MOE_DT_F16,
+            torch.bfloat16: MOE_DT_BF16}.get(t.dtype)
+    if code is None:
+        raise MoeError(MOE_ERR_INVALID, f"tensor type {t.dtype} is none of f32, f16 and bf16")
+    return code
 
 
 def _stream(stream) -> int | None:
@@ -161,6 +172,183 @@ class MoeLayerEngine:
 
     def last_launch_count(self) -> int:
         return int(lib().moe_last_launch_count(self._h))
+
+    # -- operators on device tensors (rows sorted by expert, norms of a block) --
+    def _tensor(self, name, t, shape, dtype=None):
+        """A CUDA tensor on this engine's device, of this shape (None: any) and
+        with elements of a row side by side."""
+        if not t.is_cuda or t.device.index != self.device:
+            raise MoeError(MOE_ERR_INVALID, f"{name} is on {t.device}, not cuda:{self.device}")
+        if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+            raise MoeError(MOE_ERR_INVALID, f"{name} has shape {tuple(t.shape)}, not {shape}")
+        if dtype is not None and t.dtype != dtype:
+            raise MoeError(MOE_ERR_INVALID, f"{name} is {t.dtype}, not {dtype}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise MoeError(MOE_ERR_INVALID, f"{name}: elements of a row are not side by side")
+        return t
+
+    def _ld(self, name, t, width) -> int:
+        """Row stride of a 2-D tensor (or of each matrix of a 3-D one)."""
+        ld = t.stride(-2) if t.shape[-2] > 1 else max(width, t.stride(-2))
+        if ld < width:
+            raise MoeError(MOE_ERR_INVALID, f"{name}: rows overlap (stride {ld})")
+        return ld
+
+    def _grouped(self, rows_k, rows_n, w, seg_off, result):
+        import torch
+        names, (xk, xn) = ("x", "out") if result is rows_n else ("dx", "dout"), (rows_k, rows_n)
+        if w.dim() != 3:
+            raise MoeError(MOE_ERR_INVALID, f"expert tensor has shape {tuple(w.shape)}")
+        E, n, k = w.shape
+        R = xk.shape[0]
+        self._tensor("w", w, (E, n, k))
+        self._tensor(names[0], xk, (R, k))
+        self._tensor(names[1], xn, (R, n))
+        self._tensor("seg_off", seg_off, (E + 1,), torch.int32)
+        operand = [t for t in (xk, xn, w) if t is not result]
+        if operand[0].dtype != operand[1].dtype:
+            raise MoeError(MOE_ERR_INVALID,
+                           f"operand types differ: {operand[0].dtype}, {operand[1].dtype}")
+        return MoeGroupedDesc(E, R, n, k, _dt(operand[0]), _dt(result), self._ld(names[0], xk, k),
+                              self._ld("w", w, k), w.stride(0), self._ld(names[1], xn, n))
+
+    def grouped_mm(self, x, w, seg_off, out, stream=None):
+        """out[r] = x[r] @ w[e].T for the rows r of expert e, rows sorted by
+        expert.  x [R, k], w [E, n, k], both f16 or both bf16; out [R, n] of that
+        type or f32; seg_off int32 [E + 1].  Rows outside every segment stay."""
+        d = self._grouped(x, out, w, seg_off, out)
+        self._check(lib().moe_grouped_mm(self._h, d, x.data_ptr(), w.data_ptr(),
+                                         seg_off.data_ptr(), out.data_ptr(), _stream(stream)))
+
+    def grouped_mm_dgrad(self, dout, w, seg_off, dx, stream=None):
+        """Gradient of grouped_mm's rows: dx[r] = dout[r] @ w[e]."""
+        d = self._grouped(dx, dout, w, seg_off, dx)
+        self._check(lib().moe_grouped_mm_dgrad(self._h, d, dout.data_ptr(), w.data_ptr(),
+                                               seg_off.data_ptr(), dx.data_ptr(),
+                                               _stream(stream)))
+
+    def grouped_mm_wgrad(self, dout, x, seg_off, dw, stream=None):
+        """Gradient of grouped_mm's experts: dw[e] = dout[rows].T @ x[rows], zeros
+        for an expert without rows."""
+        d = self._grouped(x, dout, dw, seg_off, dw)
+        self._check(lib().moe_grouped_mm_wgrad(self._h, d, dout.data_ptr(), x.data_ptr(),
+                                               seg_off.data_ptr(), dw.data_ptr(),
+                                               _stream(stream)))
+
+    def mxfp4_empty(self, rows: int, k: int):
+        """Uninitialised (codes, scales) of `rows` MXFP4 rows of k values."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        return (torch.empty((rows, lib().moe_mxfp4_code_stride(k)), dtype=torch.uint8, device=dev),
+                torch.empty((rows, lib().moe_mxfp4_scale_stride(k)), dtype=torch.uint8, device=dev))
+
+    def _mxfp4(self, name, codes, scales, rows, k):
+        import torch
+        L = lib()
+        for part, t, ld in (("codes", codes, L.moe_mxfp4_code_stride(k)),
+                            ("scales", scales, L.moe_mxfp4_scale_stride(k))):
+            self._tensor(f"{name} {part}", t, (rows, ld), torch.uint8)
+            if not t.is_contiguous():
+                raise MoeError(MOE_ERR_INVALID, f"{name} {part} are not contiguous")
+
+    def mxfp4_quantize(self, x, codes, scales, rows=None, stream=None):
+        """x [T, k] (f32, f16 or bf16) to MXFP4 rows (mxfp4_empty); `rows` (int32,
+        optional) names the row of x that each output row takes."""
+        import torch
+        T, k = self._tensor("x", x, (None, None)).shape
+        n = T if rows is None else self._tensor("rows", rows, (None,), torch.int32).shape[0]
+        self._mxfp4("x", codes, scales, n, k)
+        self._check(lib().moe_mxfp4_quantize(self._h, x.data_ptr(), _dt(x), self._ld("x", x, k), T,
+                                             _ptr(rows), n, k, codes.data_ptr(),
+                                             scales.data_ptr(), _stream(stream)))
+
+    def mxfp4_dequantize(self, codes, scales, out, stream=None):
+        """The values of MXFP4 rows, into out [R, k] (f32, f16 or bf16)."""
+        R, k = self._tensor("out", out, (None, None)).shape
+        self._mxfp4("row", codes, scales, R, k)
+        self._check(lib().moe_mxfp4_dequantize(self._h, codes.data_ptr(), scales.data_ptr(), R, k,
+                                               out.data_ptr(), _dt(out),
+                                               self._ld("out", out, k), _stream(stream)))
+
+    def grouped_mm_mxfp4(self, xcodes, xscales, wcodes, wscales, seg_off, k: int, out,
+                         stream=None):
+        """grouped_mm of MXFP4 rows: x [R] rows, w [E * n] rows of k values, out
+        [R, n] in f32, f16 or bf16."""
+        import torch
+        E = self._tensor("seg_off", seg_off, (None,), torch.int32).shape[0] - 1
+        R, n = self._tensor("out", out, (None, None)).shape
+        self._mxfp4("x", xcodes, xscales, R, k)
+        self._mxfp4("w", wcodes, wscales, E * n, k)
+        self._check(lib().moe_grouped_mm_mxfp4(self._h, E, R, n, k, xcodes.data_ptr(),
+                                               xscales.data_ptr(), wcodes.data_ptr(),
+                                               wscales.data_ptr(), seg_off.data_ptr(),
+                                               out.data_ptr(), _dt(out), self._ld("out", out, n),
+                                               _stream(stream)))
+
+    def _norm_desc(self, res, blk, gains, gate, post_norm, residual_scale, eps):
+        """Shared checks: res / blk are the named [T, H] tensors of the residual
+        and the block (None where absent); the tensors of a kind share type and
+        row stride."""
+        import torch
+        T, H = next(t for _, t in res if t is not None).shape
+        ld = []
+        for kind in (res, blk):
+            first = next(((s, t) for s, t in kind if t is not None), None)
+            for s, t in kind:
+                if t is None:
+                    continue
+                self._tensor(s, t, (T, H), first[1].dtype)
+                if self._ld(s, t, H) != self._ld(first[0], first[1], H):
+                    raise MoeError(MOE_ERR_INVALID, f"{s} and {first[0]}: row strides differ")
+            ld.append(None if first is None else (_dt(first[1]), self._ld(*first, H)))
+        for s, t in gains:
+            if t is not None:
+                self._tensor(s, t, (H,), torch.float32)
+        for s, t in gate:
+            if t is not None and not self._tensor(s, t, (T,), torch.float32).is_contiguous():
+                raise MoeError(MOE_ERR_INVALID, f"{s} is not contiguous")
+        (rd, rld), (bd, bld) = ld[0], ld[1] or ld[0]
+        return MoeBlockNormDesc(T, H, rd, bd, rld, bld, int(post_norm), residual_scale, eps)
+
+    def block_norm(self, x, x_out, h, w_pre=None, y=None, w_post=None, gate=None,
+                   post_norm: bool = True, residual_scale: float = 1.0, eps: float = 1e-5,
+                   stream=None):
+        """x_out = residual_scale * x + gate * norm(y) * w_post, h = norm(x_out) *
+        w_pre (RMS norms; post_norm=False adds gate * y).  x, x_out [T, H] of one
+        type; y, h [T, H] of that type, or of any when x is f32; gains f32 [H],
+        gate f32 [T]; x_out or h may be None, x_out may be x and h may be y."""
+        d = self._norm_desc([("x", x), ("x_out", x_out)], [("y", y), ("h", h)],
+                            [("w_pre", w_pre), ("w_post", w_post)], [("gate", gate)], post_norm,
+                            residual_scale, eps)
+        self._check(lib().moe_block_norm(self._h, d, x.data_ptr(), _ptr(y), _ptr(w_post),
+                                         _ptr(gate), _ptr(w_pre), _ptr(x_out), _ptr(h),
+                                         _stream(stream)))
+
+    def block_norm_backward(self, dx_out, dh, x_out, w_pre, dx, dw_pre=None, y=None, w_post=None,
+                            gate=None, dy=None, dw_post=None, dgate=None, post_norm: bool = True,
+                            residual_scale: float = 1.0, eps: float = 1e-5, stream=None):
+        """Backward pass of block_norm from its x_out and y: dx, dy and, where
+        given, the gradients of the gains (f32 [H]) and of the gate (f32 [T]).
+        dx_out or dh may be None (zeros); dx may be dx_out and dy may be dh."""
+        import torch
+        d = self._norm_desc([("x_out", x_out), ("dx_out", dx_out), ("dx", dx)],
+                            [("dh", dh), ("y", y), ("dy", dy)],
+                            [("w_pre", w_pre), ("w_post", w_post), ("dw_pre", dw_pre),
+                             ("dw_post", dw_post)], [("gate", gate), ("dgate", dgate)], post_norm,
+                            residual_scale, eps)
+        need = lib().moe_block_norm_backward_workspace(self._h, d.rows, d.hidden)
+        dev = torch.device("cuda", self.device)
+        if stream is None:
+            stream = torch.cuda.ExternalStream(lib().moe_get_stream(self._h), device=dev)
+        # from the pool of the stream that uses it, so that its reuse is ordered there
+        with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
+                               torch.cuda.ExternalStream(stream, device=dev)):
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        self._check(lib().moe_block_norm_backward(self._h, d, _ptr(dx_out), _ptr(dh),
+                                                  x_out.data_ptr(), _ptr(y), _ptr(w_post),
+                                                  _ptr(gate), _ptr(w_pre), dx.data_ptr(), _ptr(dy),
+                                                  _ptr(dw_post), _ptr(dgate), _ptr(dw_pre),
+                                                  ws.data_ptr(), need, _stream(stream)))
 
     def set_wait_limit(self, ns: int = 0):
         """Bound of the device-side waits (grid barriers, expert-parallel flag

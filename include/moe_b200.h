@@ -317,6 +317,112 @@ moe_status moe_profile_enable(moe_handle *h, int enable);
 moe_status moe_profile_read(moe_handle *h, moe_kernel_time *out, int max_entries,
                             int *n_entries);
 
+/* ------------------------------------------------------------------------
+ * 4. Operators around the router on device tensors: experts in 16-bit and in
+ *    4-bit float, and the norms of a block (no reference counterpart).  They
+ *    take explicit shapes, so one handle serves any of them; the handle gives
+ *    the device, the default stream, the error text, the status word and the
+ *    profile.  Tensors lie on the handle's device; outputs overlap no input
+ *    unless a call says so.  Calls are stream-ordered, asynchronous and may be
+ *    captured; they keep no device memory, so calls on several streams and
+ *    captured graphs are independent.  Infinities and NaNs propagate.  Types
+ *    are MOE_DT_F32, MOE_DT_F16 and MOE_DT_BF16 (below); sums are fp32 and each
+ *    result is rounded once.
+ * ---------------------------------------------------------------------- */
+/* The stream that calls with stream == NULL use. */
+void *moe_get_stream(moe_handle *h);
+
+/* Products grouped by expert.  Rows are sorted by expert: expert e owns rows
+ * [seg_off[e], seg_off[e+1]) of the [rows, .] tensors (seg_off: num_experts + 1
+ * device int32, as moe_route_permute() writes it; at most 256 experts).  Rows
+ * outside every segment are neither read nor written.  Offsets that decrease
+ * or leave [0, rows] are clamped and make moe_sync_status() report the fault.
+ * Strides are in elements.  Base addresses and row and expert strides that are
+ * multiples of 16 bytes take the tensor cores; others are computed on the SIMT
+ * pipes, many times slower. */
+typedef struct moe_grouped_desc {
+  int32_t num_experts;
+  int32_t rows;          /* R: rows of x and out; segments may cover fewer */
+  int32_t n, k;          /* w[e] is [n, k]: out[r] = x[r] w[e]^T */
+  int32_t dtype;         /* of x, w and dout: MOE_DT_F16 or MOE_DT_BF16 */
+  int32_t out_dtype;     /* of the call's result: the same, or MOE_DT_F32 */
+  int64_t ld_x;          /* row stride of x and dx, [rows, k] */
+  int64_t ld_w;          /* row stride of w and dw, [num_experts, n, k] */
+  int64_t expert_stride; /* of w and dw */
+  int64_t ld_out;        /* row stride of out and dout, [rows, n] */
+} moe_grouped_desc;
+/* out[r] = x[r] w[e]^T for every row r of expert e. */
+moe_status moe_grouped_mm(moe_handle *h, const moe_grouped_desc *d, const void *d_x,
+                          const void *d_w, const int32_t *d_seg_off, void *d_out, void *stream);
+/* dx[r] = dout[r] w[e]. */
+moe_status moe_grouped_mm_dgrad(moe_handle *h, const moe_grouped_desc *d, const void *d_dout,
+                                const void *d_w, const int32_t *d_seg_off, void *d_dx,
+                                void *stream);
+/* dw[e] = dout[rows of e]^T x[rows of e]; zeros for an expert without rows. */
+moe_status moe_grouped_mm_wgrad(moe_handle *h, const moe_grouped_desc *d, const void *d_dout,
+                                const void *d_x, const int32_t *d_seg_off, void *d_dw,
+                                void *stream);
+
+/* MXFP4: 32 consecutive values of a row share a power-of-two scale
+ * s = 2^(floor(log2 max|x|) - 2), at least 2^-127, held as the byte
+ * log2(s) + 127 (E8M0); each value is x / s rounded to the nearest of
+ * 0 0.5 1 1.5 2 3 4 6 with its sign (E2M1, ties to the even code, 6 past it).
+ * A block with an infinity or a NaN gets the scale byte 255 and decodes to
+ * NaN.  A row of k values is moe_mxfp4_code_stride(k) = 16 ceil(k / 32) bytes of
+ * codes, value 2i in the low nibble, and moe_mxfp4_scale_stride(k) =
+ * 4 ceil(k / 128) bytes of scales, unused ones zero.  Codes are aligned to 16
+ * bytes, scales to 4. */
+size_t moe_mxfp4_code_stride(int k);
+size_t moe_mxfp4_scale_stride(int k);
+/* Quantise `rows` rows of k values.  d_index (optional, [rows] device int32)
+ * names the source row of each, e.g. a route's token; a row whose index is
+ * outside [0, src_rows) becomes zeros and moe_sync_status() reports it. */
+moe_status moe_mxfp4_quantize(moe_handle *h, const void *d_x, int dtype, int64_t ld_x,
+                              int src_rows, const int32_t *d_index, int rows, int k,
+                              uint8_t *d_codes, uint8_t *d_scales, void *stream);
+/* The values that the codes stand for. */
+moe_status moe_mxfp4_dequantize(moe_handle *h, const uint8_t *d_codes, const uint8_t *d_scales,
+                                int rows, int k, void *d_out, int dtype, int64_t ld_out,
+                                void *stream);
+/* moe_grouped_mm() of MXFP4 operands: x [rows], w [num_experts * n] rows. */
+moe_status moe_grouped_mm_mxfp4(moe_handle *h, int num_experts, int rows, int n, int k,
+                                const uint8_t *d_xcodes, const uint8_t *d_xscales,
+                                const uint8_t *d_wcodes, const uint8_t *d_wscales,
+                                const int32_t *d_seg_off, void *d_out, int out_dtype,
+                                int64_t ld_out, void *stream);
+
+/* The norms before and after a block, with its gate and the residual scale:
+ *   z     = y / rms(y) * w_post         (post_norm 0: z = y)
+ *   x_out = residual_scale * x + gate * z
+ *   h     = x_out / rms(x_out) * w_pre  (input of the next block)
+ * with rms(v) = sqrt(sum v^2 / hidden + eps).  Without y only the norm before
+ * the first block remains.  Gains and gates are f32: w_post, w_pre [hidden]
+ * (NULL = ones), gate [rows] (NULL = 1).  x_out or h may be NULL; x_out may be
+ * x and h may be y. */
+typedef struct moe_block_norm_desc {
+  int32_t rows, hidden;   /* hidden <= 16384 */
+  int32_t res_dtype;      /* of x, x_out, dx_out, dx */
+  int32_t dtype;          /* of y, h, dh, dy: res_dtype, or any type when that is F32 */
+  int64_t ld_res, ld_block; /* row strides of the two kinds, in elements */
+  int32_t post_norm;
+  float residual_scale, eps;
+} moe_block_norm_desc;
+moe_status moe_block_norm(moe_handle *h, const moe_block_norm_desc *d, const void *d_x,
+                          const void *d_y, const float *d_w_post, const float *d_gate,
+                          const float *d_w_pre, void *d_x_out, void *d_h, void *stream);
+/* Its backward pass from x_out and y.  dx_out or dh may be NULL (zeros); dy
+ * comes with y; dw_post, dgate and dw_pre are optional.  dx may be dx_out and
+ * dy may be dh.  The gains' gradients are sums over the rows in an order fixed
+ * by the shape; the workspace (4-byte aligned device memory that no other call
+ * uses meanwhile) holds their parts. */
+size_t moe_block_norm_backward_workspace(const moe_handle *h, int rows, int hidden);
+moe_status moe_block_norm_backward(moe_handle *h, const moe_block_norm_desc *d,
+                                   const void *d_dx_out, const void *d_dh, const void *d_x_out,
+                                   const void *d_y, const float *d_w_post, const float *d_gate,
+                                   const float *d_w_pre, void *d_dx, void *d_dy,
+                                   float *d_dw_post, float *d_dgate, float *d_dw_pre,
+                                   void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* ---- Merged-INT8 checkpoints --------------------------------------------
  * The safetensors shards written by the reference's converter
  * (tools/prepare_olmoe.py:85-94): per expert
