@@ -26,6 +26,9 @@ struct GroupedArgs {
 };
 
 cudaError_t launch_grouped_simple(GroupedKind kind, const GroupedArgs &a, cudaStream_t s);
+// The tensor-core form, for 16-byte aligned operands (grouped_tc_ok).
+bool grouped_tc_ok(GroupedKind kind, const GroupedArgs &a);
+cudaError_t launch_grouped_tc(GroupedKind kind, const GroupedArgs &a, cudaStream_t s);
 
 // ---- MXFP4 ---------------------------------------------------------------
 struct Mxfp4Quant {

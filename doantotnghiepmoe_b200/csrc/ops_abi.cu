@@ -80,7 +80,10 @@ moe_status run_grouped(moe_handle *h, GroupedKind kind, const char *name, Groupe
     return MOE_OK;
   }
   return launch(h, name, stream, 1,
-                [&](cudaStream_t s) { return launch_grouped_simple(kind, a, s); });
+                [&](cudaStream_t s) {
+                  return grouped_tc_ok(kind, a) ? launch_grouped_tc(kind, a, s)
+                                                : launch_grouped_simple(kind, a, s);
+                });
 }
 
 }  // namespace
