@@ -22,8 +22,6 @@
 
 #include <algorithm>
 
-#include "../../include/moe_b200.h"
-#include "cvt.cuh"
 #include "expert_tc.h"
 #include "ops.h"
 #include "segments.cuh"
@@ -214,28 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint32_t trow =
           pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16);
-      for (int c = grp * 32; c < it.nc; c += 64) {
-        uint32_t v[32];
-        if (some) {
-          tmem_ld32(trow + c, v);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0;
-        }
-        if (m < M) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (c + i >= it.nc) break;
-            const int64_t at = at0 + (c + i) * ld;
-            const float f = __uint_as_float(v[i]);
-            if (a.out_dtype == MOE_DT_F32) reinterpret_cast<float *>(a.out)[at] = f;
-            else if (a.out_dtype == MOE_DT_BF16)
-              reinterpret_cast<__nv_bfloat16 *>(a.out)[at] = from_f32<__nv_bfloat16>(f);
-            else reinterpret_cast<__half *>(a.out)[at] = from_f32<__half>(f);
-          }
-        }
-      }
+      drain_tile(trow, some, it.nc, grp, m < M, a.out, a.out_dtype, at0, ld);
       if (some) {
         fence_before_sync();
         __syncwarp();

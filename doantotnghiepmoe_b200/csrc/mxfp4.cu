@@ -19,9 +19,9 @@
 #include <algorithm>
 
 #include "../../include/moe_b200.h"
+#include "common.cuh"
 #include "cvt.cuh"
 #include "ops.h"
-#include "segments.cuh"
 
 namespace moe {
 namespace {
@@ -152,40 +152,6 @@ cudaError_t dequantize_t(const Mxfp4Dequant &a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// ---------------------------------------------------------------------------
-// Grouped product of MXFP4 operands: each thread of a 16 x 16 block owns one
-// output value and decodes its operands as it goes.
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) mxfp4_mm_simple_kernel(Mxfp4Args a) {
-  __shared__ SegTable seg;
-  if (threadIdx.x < 32) build_segments(seg, a.seg_off, a.E, a.R, 16, a.status);
-  __syncthreads();
-  const int ldc = mxfp4_code_stride(a.k), lds = mxfp4_scale_stride(a.k), nb = (a.k + 31) / 32;
-  const int tj = (a.n + 15) / 16;
-  for (long long it = blockIdx.x; it < (long long)seg.total * tj; it += gridDim.x) {
-    const int j = (int)(it % tj) * 16 + threadIdx.x % 16, g = (int)(it / tj);
-    const int e = seg.expert_of(g, a.E);
-    const int i = (g - seg.tile0[e]) * 16 + threadIdx.x / 16;
-    if (i >= seg.rows(e) || j >= a.n) continue;
-    const int64_t r = seg.off[e] + i, wr = (int64_t)e * a.n + j;
-    float acc = 0.0f;
-    for (int b = 0; b < nb; ++b) {
-      float dot = 0.0f;
-      for (int q = 0; q < 16; ++q) {
-        const uint32_t cx = a.xc[r * ldc + b * 16 + q], cw = a.wc[wr * ldc + b * 16 + q];
-        dot = fmaf(e2m1_value(cx & 15u), e2m1_value(cw & 15u), dot);
-        dot = fmaf(e2m1_value(cx >> 4), e2m1_value(cw >> 4), dot);
-      }
-      acc = fmaf(dot * e8m0_value(a.xs[r * lds + b]), e8m0_value(a.ws[wr * lds + b]), acc);
-    }
-    const int64_t at = r * a.ld_out + j;
-    if (a.out_dtype == MOE_DT_F32) reinterpret_cast<float *>(a.out)[at] = acc;
-    else if (a.out_dtype == MOE_DT_BF16)
-      reinterpret_cast<__nv_bfloat16 *>(a.out)[at] = from_f32<__nv_bfloat16>(acc);
-    else reinterpret_cast<__half *>(a.out)[at] = from_f32<__half>(acc);
-  }
-}
-
 }  // namespace
 
 cudaError_t launch_mxfp4_quantize(const Mxfp4Quant &a, cudaStream_t s) {
@@ -198,12 +164,6 @@ cudaError_t launch_mxfp4_dequantize(const Mxfp4Dequant &a, cudaStream_t s) {
   if (a.rows <= 0) return cudaSuccess;
   if (a.dtype == MOE_DT_F32) return dequantize_t<float>(a, s);
   return a.dtype == MOE_DT_BF16 ? dequantize_t<__nv_bfloat16>(a, s) : dequantize_t<__half>(a, s);
-}
-
-cudaError_t launch_mxfp4_mm_simple(const Mxfp4Args &a, cudaStream_t s) {
-  if (a.R <= 0) return cudaSuccess;
-  mxfp4_mm_simple_kernel<<<a.sm_count * 8, 256, 0, s>>>(a);
-  return cudaGetLastError();
 }
 
 }  // namespace moe

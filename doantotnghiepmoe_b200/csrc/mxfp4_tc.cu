@@ -1,0 +1,231 @@
+// Grouped product of MXFP4 operands on the tensor cores: out[r, m] = sum over
+// the blocks b of K of sx[r, b] sw[m, b] <qx[r, b], qw[m, b]> as
+// tcgen05.mma kind::mxf4, which takes the 4-bit codes and the scale bytes as
+// they lie in memory and adds in fp32: nothing is decoded.
+//
+// The shape of the kernel is that of grouped_tc.cu: weights on the M side,
+// an expert's rows on the N side in tiles that are any multiple of 16, one
+// persistent CTA an SM, a ring of TMA stages that runs on across items, two
+// accumulator buffers.  A stage is 256 elements of K: 128-byte rows of codes
+// of 128 weight rows and up to 192 rows of x.
+//
+// The MMA reads the scales from TMEM, one 32-bit column for 32 rows and 4
+// blocks (128 elements of K), in the order of the rows' lanes.  Scale bytes
+// lie by row in memory; four warps, each at another stage, fetch 4 of them at
+// a time and store them in the order that a 32-row copy to TMEM takes: word
+// (r % 32) * 4 + r / 32 of a 512-byte group.  192 rows of N rather than 256 leave room in TMEM for four
+// sets of scales beside the two buffers, so that a set is written again only
+// after the MMAs that read it are known to be done.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "expert_tc.h"
+#include "ops.h"
+#include "segments.cuh"
+#include "tc_ptx.cuh"
+
+namespace moe {
+namespace {
+
+using namespace tcp;
+
+constexpr int kTM = 128, kTN = 192;
+constexpr int kStages = 5, kSets = 4;
+constexpr uint32_t kABytes = kTM * 128, kBBytes = kTN * 128, kStageBytes = kABytes + kBBytes;
+constexpr int kBoxRows = 32;
+constexpr int kGroup = 512;            // scale bytes of 128 rows and 4 blocks
+constexpr int kScaleBytes = 6 * kGroup;  // of a stage: 2 groups of w, 2 x 2 of x
+constexpr int kSetCols = 24;             // TMEM columns of a stage's scales
+constexpr uint32_t kTmemCols = 512;
+static_assert(2 * kTN + kSets * kSetCols <= (int)kTmemCols, "TMEM");
+constexpr int kScaleWarps = 4;
+constexpr int kMxThreads = kThreads + 32 * kScaleWarps;
+constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
+                         (size_t)kStages * (kStageBytes + kScaleBytes);
+static_assert(kSmem <= 232448, "shared memory");
+
+__global__ void __launch_bounds__(kMxThreads, 1)
+    mxfp4_tc_kernel(const __grid_constant__ CUtensorMap mapW,
+                    const __grid_constant__ CUtensorMap mapX, Mxfp4Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  using P = Pipe<kStages>;
+  P &pp = *reinterpret_cast<P *>(smem_raw);
+  SegTable &seg = *reinterpret_cast<SegTable *>(smem_raw + sizeof(P));
+  uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
+  uint8_t *scales = tiles + kStages * kStageBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) pp.init(1 + 32);  // the copying thread, a scale warp's lanes
+  if (warp == 1) tmem_alloc(&pp.tmem_base, kTmemCols);
+  if (warp == 2) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+
+  const int nM = (a.n + kTM - 1) / kTM, nk = (a.k + 255) / 256;
+  const long long total = (long long)seg.total * nM;
+  struct Item {
+    int e, m0, c0, nc;
+  };
+  const auto item = [&](long long w) {
+    Item it;
+    it.m0 = (int)(w % nM) * kTM;
+    const int g = (int)(w / nM);
+    it.e = seg.expert_of(g, a.E);
+    const int cnt = seg.rows(it.e), nt = seg.tile0[it.e + 1] - seg.tile0[it.e];
+    const int sz = tile_rows(cnt, nt), t = g - seg.tile0[it.e];
+    it.c0 = seg.off[it.e] + t * sz;
+    it.nc = min(sz, cnt - t * sz);
+    return it;
+  };
+
+  if (warp == 0 && lane == 0) {
+    int q = 0;
+    for (long long w = blockIdx.x; w < total && !pp.abort_flag; w += gridDim.x) {
+      const Item it = item(w);
+      const int nbox = (it.nc + kBoxRows - 1) / kBoxRows;
+      for (int kb = 0; kb < nk; ++kb, ++q) {
+        const int s = q % kStages, use = q / kStages;
+        if (use > 0 && !tma::mbar_wait(&pp.empty[s], (use - 1) & 1, &pp.abort_flag)) {
+          pp.abort_flag = 1;
+          break;
+        }
+        uint8_t *st = tiles + s * kStageBytes;
+        tma::mbar_expect_tx(&pp.full[s], kABytes + nbox * kBoxRows * 128u);
+        tma::load_3d(st, &mapW, &pp.full[s], kb * 128, it.m0, it.e);
+        for (int i = 0; i < nbox; ++i)
+          tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapX, &pp.full[s], kb * 128,
+                       it.c0 + i * kBoxRows, 0);
+      }
+    }
+    if (pp.abort_flag) {  // issued stages must land before the CTA may exit
+      const int from = *(volatile int *)&pp.consumed;
+      for (int k = from; k < q; ++k)
+        tma::mbar_wait(&pp.full[k % kStages], (k / kStages) & 1, nullptr, tma::kWaitCycles / 64);
+    }
+  } else if (warp == 1) {
+    // E2M1 operands, E8M0 scales, M = 128
+    const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kTM >> 4) << 24);
+    const uint32_t sf0 = pp.tmem_base + 2 * kTN;
+    int q = 0, j = 0;
+    for (long long w = blockIdx.x; w < total; w += gridDim.x, ++j) {
+      const Item it = item(w);
+      const int buf = j & 1;
+      if (j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
+      fence_after_sync();
+      const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
+      const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 15) >> 4) << 18);
+      const int rgroups = (it.nc + 127) / 128;
+      bool ok = true;
+      for (int kb = 0; kb < nk; ++kb, ++q) {
+        const int s = q % kStages;
+        // the MMAs that read this set of scales are done
+        if (q >= kSets) {
+          const int p = q - kSets;
+          ok = pp.wait_warp(&pp.empty[p % kStages], (p / kStages) & 1);
+        }
+        if (!ok || !pp.wait_warp(&pp.full[s], (q / kStages) & 1)) {
+          ok = false;
+          break;
+        }
+        fence_after_sync();
+        if (lane == 0) {
+          const uint32_t base = su32(tiles + s * kStageBytes);
+          const uint32_t sb = su32(scales + s * kScaleBytes);
+          const uint32_t sfa = sf0 + (uint32_t)(q % kSets) * kSetCols, sfb = sfa + 8;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            cp_scales(sfa + 4 * g, rows16_desc(sb + g * kGroup));
+            for (int r = 0; r < rgroups; ++r)
+              cp_scales(sfb + 8 * g + 4 * r, rows16_desc(sb + (2 + 2 * g + r) * kGroup));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t id = (uint32_t)(k & 1) * 2;  // bytes 0-1 or 2-3 of a scale word
+            mma_mxf4(d, sw128_desc(base + k * 32, 16, 1024),
+                     sw128_desc(base + kABytes + k * 32, 16, 1024), idesc | (id << 4) | (id << 29),
+                     sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
+          }
+          commit(&pp.empty[s]);
+          pp.consumed = q + 1;
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (lane == 0) commit(&pp.tfull[buf]);
+    }
+    if (lane == 0) commit(&pp.done);
+  } else if (warp >= 2 && warp < 2 + kScaleWarps) {
+    const int words = mxfp4_scale_stride(a.k) / 4;
+    const uint32_t *xs = reinterpret_cast<const uint32_t *>(a.xs);
+    const uint32_t *ws = reinterpret_cast<const uint32_t *>(a.ws);
+    long long w = blockIdx.x;
+    int kb = warp - 2;  // this warp's steps: every kScaleWarps-th
+    for (int q = warp - 2;; q += kScaleWarps, kb += kScaleWarps) {
+      for (; kb >= nk && w < total; kb -= nk) w += gridDim.x;
+      if (w >= total) break;
+      const Item it = item(w);
+      // v[g]: the words of rows l, l + 32, l + 64, l + 96 of w, then of x twice
+      uint32_t v[2][12];
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        const int r = i % 4 * 32 + (i < 8 ? 0 : 128) + lane;
+        const bool in = i < 4 ? it.m0 + r < a.n : r < it.nc;
+        const uint32_t *row = i < 4 ? ws + ((int64_t)it.e * a.n + it.m0 + r) * words
+                                    : xs + ((int64_t)it.c0 + r) * words;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          v[g][i] = in && 2 * kb + g < words ? __ldg(row + 2 * kb + g) : 0u;
+      }
+      const int s = q % kStages, use = q / kStages;
+      if (use > 0 && !pp.wait_warp(&pp.empty[s], (use - 1) & 1)) break;
+      uint4 *dst = reinterpret_cast<uint4 *>(scales + s * kScaleBytes) + lane;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        dst[g * 32] = make_uint4(v[g][0], v[g][1], v[g][2], v[g][3]);
+        dst[(2 + 2 * g) * 32] = make_uint4(v[g][4], v[g][5], v[g][6], v[g][7]);
+        dst[(3 + 2 * g) * 32] = make_uint4(v[g][8], v[g][9], v[g][10], v[g][11]);
+      }
+      tma::fence_proxy_async_smem();  // before the tensor cores' proxy reads them
+      tma::mbar_arrive(&pp.full[s]);
+    }
+  } else if (warp >= 2) {
+    const int ew = warp - 2 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
+    int j = 0;
+    for (long long w = blockIdx.x; w < total; w += gridDim.x, ++j) {
+      const Item it = item(w);
+      const int m = it.m0 + quarter * 32 + lane, buf = j & 1;
+      if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
+      fence_after_sync();
+      drain_tile(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), true,
+                 it.nc, grp, m < a.n, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out);
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tma::mbar_arrive(&pp.tempty[buf]);
+    }
+  }
+  if (threadIdx.x == 32) tma::mbar_wait(&pp.done, 0, nullptr);  // no MMA still runs
+  fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && pp.abort_flag) set_status(a.status, kStatusTimeout);
+  if (warp == 1) tmem_dealloc(pp.tmem_base, kTmemCols);
+}
+
+}  // namespace
+
+cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
+  if (a.R <= 0) return cudaSuccess;
+  static const cudaError_t attr = cudaFuncSetAttribute(
+      mxfp4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+  if (attr != cudaSuccess) return attr;
+  const uint64_t row = (uint64_t)mxfp4_code_stride(a.k);
+  CUtensorMap w, x;
+  if (!tc::encode_map3d(&w, a.wc, row, (uint64_t)a.n, (uint64_t)a.E, row, row * a.n, kTM) ||
+      !tc::encode_map3d(&x, a.xc, row, (uint64_t)a.R, 1, row, row, kBoxRows))
+    return cudaErrorInvalidValue;
+  const long long items = (long long)(a.R / kTN + std::min(a.E, a.R)) * ((a.n + kTM - 1) / kTM);
+  mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(w, x, a);
+  return cudaGetLastError();
+}
+
+}  // namespace moe

@@ -63,7 +63,7 @@ constexpr int mxfp4_scale_stride(int k) { return (k + 127) / 128 * 4; }
 
 cudaError_t launch_mxfp4_quantize(const Mxfp4Quant &a, cudaStream_t s);
 cudaError_t launch_mxfp4_dequantize(const Mxfp4Dequant &a, cudaStream_t s);
-cudaError_t launch_mxfp4_mm_simple(const Mxfp4Args &a, cudaStream_t s);
+cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s);
 
 // ---- norms around a block --------------------------------------------------
 struct BlockNormArgs {

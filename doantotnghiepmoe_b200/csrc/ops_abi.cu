@@ -211,7 +211,7 @@ extern "C" moe_status moe_grouped_mm_mxfp4(moe_handle *h, int num_experts, int r
   h->last_launches = 0;
   if (rows == 0) return MOE_OK;
   return launch(h, "grouped_mm_mxfp4", stream, 1,
-                [&](cudaStream_t s) { return launch_mxfp4_mm_simple(a, s); });
+                [&](cudaStream_t s) { return launch_mxfp4_mm(a, s); });
 }
 
 // ---------------------------------------------------------------------------

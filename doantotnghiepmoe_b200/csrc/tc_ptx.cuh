@@ -5,7 +5,9 @@
 
 #include <cstdint>
 
+#include "../../include/moe_b200.h"
 #include "common.cuh"
+#include "cvt.cuh"
 #include "tma_ptx.cuh"
 
 namespace moe {
@@ -47,6 +49,24 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D (+)= (A sA) (B sB)^T of E2M1 operands with an E8M0 scale for 32 elements of
+// K, fp32 sums; 64 elements of K.  sfa / sfb: TMEM columns of the scales.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, "
+      "[%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 32 rows of 16 bytes of shared memory into 4 TMEM columns, the same in each
+// quarter of the lanes; ordered before later MMAs of this thread.
+__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc)
+               : "memory");
+}
 // 32 accumulator columns of this warp's 32 TMEM lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
@@ -71,6 +91,12 @@ __device__ __forceinline__ void tmem_wait_ld() {
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) |
          ((uint64_t)(sbo >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Descriptor of 32 rows of 16 bytes back to back (no swizzle): groups of 8 rows
+// 128 bytes apart.
+__device__ __forceinline__ uint64_t rows16_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 
 constexpr int kEpiWarps = 8;                   // two a TMEM lane quarter
@@ -110,6 +136,37 @@ struct Pipe {
 
 __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
   return reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+}
+
+// Writes a tile's sums: column c of the accumulator is row c of the result,
+// and lane l of a quarter its element m0 + l.  Called by the 8 draining warps,
+// grp the half of the columns (in turns of 32) that this warp takes.
+template <typename T>
+__device__ __forceinline__ void store_cols(T *out, int64_t ld, int c, int nc,
+                                           const uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (c + i < nc) out[(c + i) * ld] = from_f32<T>(__uint_as_float(v[i]));
+}
+__device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int grp, bool inside,
+                                           void *out, int out_dtype, int64_t at, int64_t ld) {
+  for (int c = grp * 32; c < nc; c += 64) {
+    uint32_t v[32];
+    if (some) {
+      tmem_ld32(trow + c, v);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0;
+    }
+    if (inside) {
+      if (out_dtype == MOE_DT_F32) store_cols(reinterpret_cast<float *>(out) + at, ld, c, nc, v);
+      else if (out_dtype == MOE_DT_BF16)
+        store_cols(reinterpret_cast<__nv_bfloat16 *>(out) + at, ld, c, nc, v);
+      else store_cols(reinterpret_cast<__half *>(out) + at, ld, c, nc, v);
+    }
+    __syncwarp();  // the next load is the whole warp's
+  }
 }
 
 // Rows of the t-th of nt row tiles of an expert with cnt rows: equal tiles, a

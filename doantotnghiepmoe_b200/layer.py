@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import cached_property
 
 import numpy as np
 
@@ -33,20 +34,41 @@ def _ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_DTYPES: dict = {}
+
+
 def _dt(t) -> int:
     """MOE_DT_* of a floating-point tensor."""
-    import torch
-    code = {torch.float32: MOE_DT_F32, torch.float16: MOE_DT_F16,
-            torch.bfloat16: MOE_DT_BF16}.get(t.dtype)
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: MOE_DT_F32, torch.float16: MOE_DT_F16,
+                        torch.bfloat16: MOE_DT_BF16})
+    code = _DTYPES.get(t.dtype)
     if code is None:
         raise MoeError(MOE_ERR_INVALID, f"tensor type {t.dtype} is none of f32, f16 and bf16")
     return code
+
+
+def mxfp4_strides(k: int) -> tuple:
+    """Bytes of codes and of scales of an MXFP4 row of k values
+    (moe_mxfp4_code_stride, moe_mxfp4_scale_stride)."""
+    return (k + 31) // 32 * 16, (k + 127) // 128 * 4
 
 
 def _stream(stream) -> int | None:
     if stream is None:
         return None
     return getattr(stream, "cuda_stream", stream)
+
+
+def _op_stream(stream) -> int | None:
+    """The stream argument of an operator call: None is the handle's stream, a
+    torch stream that stream itself -- torch's default stream has the handle 0,
+    which the C ABI takes for the handle's stream, so it is named by
+    cudaStreamLegacy."""
+    if stream is None:
+        return None
+    return getattr(stream, "cuda_stream", stream) or 1
 
 
 class MoeLayerEngine:
@@ -174,43 +196,52 @@ class MoeLayerEngine:
         return int(lib().moe_last_launch_count(self._h))
 
     # -- operators on device tensors (rows sorted by expert, norms of a block) --
-    def _tensor(self, name, t, shape, dtype=None):
-        """A CUDA tensor on this engine's device, of this shape (None: any) and
-        with elements of a row side by side."""
-        if not t.is_cuda or t.device.index != self.device:
-            raise MoeError(MOE_ERR_INVALID, f"{name} is on {t.device}, not cuda:{self.device}")
-        if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-            raise MoeError(MOE_ERR_INVALID, f"{name} has shape {tuple(t.shape)}, not {shape}")
-        if dtype is not None and t.dtype != dtype:
-            raise MoeError(MOE_ERR_INVALID, f"{name} is {t.dtype}, not {dtype}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise MoeError(MOE_ERR_INVALID, f"{name}: elements of a row are not side by side")
-        return t
+    @cached_property
+    def _dev(self):
+        import torch
+        return torch.device("cuda", self.device)
 
-    def _ld(self, name, t, width) -> int:
-        """Row stride of a 2-D tensor (or of each matrix of a 3-D one)."""
-        ld = t.stride(-2) if t.shape[-2] > 1 else max(width, t.stride(-2))
+    def _bad(self, name, t, want):
+        raise MoeError(MOE_ERR_INVALID, f"{name}: {want} on cuda:{self.device} wanted, got "
+                       f"{t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}")
+
+    def _rows(self, name, t, R, width) -> int:
+        """Row stride of t [R, width] on this engine's device, the elements of
+        a row side by side and its rows apart."""
+        if t.device != self._dev or t.shape != (R, width):
+            self._bad(name, t, f"[{R}, {width}]")
+        ld, step = t.stride()
+        if step != 1 and width > 1:
+            self._bad(name, t, "rows of adjacent elements")
         if ld < width:
-            raise MoeError(MOE_ERR_INVALID, f"{name}: rows overlap (stride {ld})")
+            if R > 1:
+                self._bad(name, t, "rows that do not overlap")
+            ld = width
         return ld
+
+    def _vec(self, name, t, n, dtype):
+        """t [n] of this type, contiguous, on this engine's device; None passes."""
+        if t is not None and (t.dtype != dtype or t.device != self._dev or t.shape != (n,) or
+                              (n > 1 and t.stride(0) != 1)):
+            self._bad(name, t, f"contiguous {dtype} [{n}]")
 
     def _grouped(self, rows_k, rows_n, w, seg_off, result):
         import torch
-        names, (xk, xn) = ("x", "out") if result is rows_n else ("dx", "dout"), (rows_k, rows_n)
-        if w.dim() != 3:
-            raise MoeError(MOE_ERR_INVALID, f"expert tensor has shape {tuple(w.shape)}")
+        xname, oname = ("x", "out") if result is rows_n else ("dx", "dout")
+        if w.dim() != 3 or rows_k.dim() != 2 or w.device != self._dev:
+            self._bad("w", w, "[experts, n, k]")
         E, n, k = w.shape
-        R = xk.shape[0]
-        self._tensor("w", w, (E, n, k))
-        self._tensor(names[0], xk, (R, k))
-        self._tensor(names[1], xn, (R, n))
-        self._tensor("seg_off", seg_off, (E + 1,), torch.int32)
-        operand = [t for t in (xk, xn, w) if t is not result]
-        if operand[0].dtype != operand[1].dtype:
-            raise MoeError(MOE_ERR_INVALID,
-                           f"operand types differ: {operand[0].dtype}, {operand[1].dtype}")
-        return MoeGroupedDesc(E, R, n, k, _dt(operand[0]), _dt(result), self._ld(names[0], xk, k),
-                              self._ld("w", w, k), w.stride(0), self._ld(names[1], xn, n))
+        R = rows_k.shape[0]
+        es, ld, step = w.stride()
+        if (step != 1 and k > 1) or (ld < k and n > 1):
+            self._bad("w", w, "rows of adjacent elements that do not overlap")
+        self._vec("seg_off", seg_off, E + 1, torch.int32)
+        p, q = (rows_k, rows_n) if result is w else \
+            (rows_k, w) if result is rows_n else (rows_n, w)
+        if p.dtype != q.dtype:
+            raise MoeError(MOE_ERR_INVALID, f"operand types differ: {p.dtype}, {q.dtype}")
+        return MoeGroupedDesc(E, R, n, k, _dt(p), _dt(result), self._rows(xname, rows_k, R, k),
+                              max(ld, k), es, self._rows(oname, rows_n, R, n))
 
     def grouped_mm(self, x, w, seg_off, out, stream=None):
         """out[r] = x[r] @ w[e].T for the rows r of expert e, rows sorted by
@@ -218,14 +249,14 @@ class MoeLayerEngine:
         type or f32; seg_off int32 [E + 1].  Rows outside every segment stay."""
         d = self._grouped(x, out, w, seg_off, out)
         self._check(lib().moe_grouped_mm(self._h, d, x.data_ptr(), w.data_ptr(),
-                                         seg_off.data_ptr(), out.data_ptr(), _stream(stream)))
+                                         seg_off.data_ptr(), out.data_ptr(), _op_stream(stream)))
 
     def grouped_mm_dgrad(self, dout, w, seg_off, dx, stream=None):
         """Gradient of grouped_mm's rows: dx[r] = dout[r] @ w[e]."""
         d = self._grouped(dx, dout, w, seg_off, dx)
         self._check(lib().moe_grouped_mm_dgrad(self._h, d, dout.data_ptr(), w.data_ptr(),
                                                seg_off.data_ptr(), dx.data_ptr(),
-                                               _stream(stream)))
+                                               _op_stream(stream)))
 
     def grouped_mm_wgrad(self, dout, x, seg_off, dw, stream=None):
         """Gradient of grouped_mm's experts: dw[e] = dout[rows].T @ x[rows], zeros
@@ -233,82 +264,87 @@ class MoeLayerEngine:
         d = self._grouped(x, dout, dw, seg_off, dw)
         self._check(lib().moe_grouped_mm_wgrad(self._h, d, dout.data_ptr(), x.data_ptr(),
                                                seg_off.data_ptr(), dw.data_ptr(),
-                                               _stream(stream)))
+                                               _op_stream(stream)))
 
     def mxfp4_empty(self, rows: int, k: int):
         """Uninitialised (codes, scales) of `rows` MXFP4 rows of k values."""
         import torch
-        dev = torch.device("cuda", self.device)
-        return (torch.empty((rows, lib().moe_mxfp4_code_stride(k)), dtype=torch.uint8, device=dev),
-                torch.empty((rows, lib().moe_mxfp4_scale_stride(k)), dtype=torch.uint8, device=dev))
+        lc, ls = mxfp4_strides(k)
+        return (torch.empty((rows, lc), dtype=torch.uint8, device=self._dev),
+                torch.empty((rows, ls), dtype=torch.uint8, device=self._dev))
 
     def _mxfp4(self, name, codes, scales, rows, k):
         import torch
-        L = lib()
-        for part, t, ld in (("codes", codes, L.moe_mxfp4_code_stride(k)),
-                            ("scales", scales, L.moe_mxfp4_scale_stride(k))):
-            self._tensor(f"{name} {part}", t, (rows, ld), torch.uint8)
-            if not t.is_contiguous():
-                raise MoeError(MOE_ERR_INVALID, f"{name} {part} are not contiguous")
+        for t, ld in zip((codes, scales), mxfp4_strides(k)):
+            if (t.dtype != torch.uint8 or t.device != self._dev or t.shape != (rows, ld) or
+                    not t.is_contiguous()):
+                self._bad(name, t, f"contiguous uint8 [{rows}, {ld}]")
 
     def mxfp4_quantize(self, x, codes, scales, rows=None, stream=None):
         """x [T, k] (f32, f16 or bf16) to MXFP4 rows (mxfp4_empty); `rows` (int32,
         optional) names the row of x that each output row takes."""
         import torch
-        T, k = self._tensor("x", x, (None, None)).shape
-        n = T if rows is None else self._tensor("rows", rows, (None,), torch.int32).shape[0]
-        self._mxfp4("x", codes, scales, n, k)
-        self._check(lib().moe_mxfp4_quantize(self._h, x.data_ptr(), _dt(x), self._ld("x", x, k), T,
-                                             _ptr(rows), n, k, codes.data_ptr(),
-                                             scales.data_ptr(), _stream(stream)))
+        if x.dim() != 2:
+            self._bad("x", x, "[T, k]")
+        T, k = x.shape
+        n = T if rows is None else rows.shape[0]
+        self._vec("rows", rows, n, torch.int32)
+        self._mxfp4("MXFP4 rows of x", codes, scales, n, k)
+        self._check(lib().moe_mxfp4_quantize(self._h, x.data_ptr(), _dt(x),
+                                             self._rows("x", x, T, k), T, _ptr(rows), n, k,
+                                             codes.data_ptr(), scales.data_ptr(),
+                                             _op_stream(stream)))
 
     def mxfp4_dequantize(self, codes, scales, out, stream=None):
         """The values of MXFP4 rows, into out [R, k] (f32, f16 or bf16)."""
-        R, k = self._tensor("out", out, (None, None)).shape
-        self._mxfp4("row", codes, scales, R, k)
+        if out.dim() != 2:
+            self._bad("out", out, "[R, k]")
+        R, k = out.shape
+        self._mxfp4("MXFP4 rows", codes, scales, R, k)
         self._check(lib().moe_mxfp4_dequantize(self._h, codes.data_ptr(), scales.data_ptr(), R, k,
                                                out.data_ptr(), _dt(out),
-                                               self._ld("out", out, k), _stream(stream)))
+                                               self._rows("out", out, R, k), _op_stream(stream)))
 
     def grouped_mm_mxfp4(self, xcodes, xscales, wcodes, wscales, seg_off, k: int, out,
                          stream=None):
         """grouped_mm of MXFP4 rows: x [R] rows, w [E * n] rows of k values, out
         [R, n] in f32, f16 or bf16."""
         import torch
-        E = self._tensor("seg_off", seg_off, (None,), torch.int32).shape[0] - 1
-        R, n = self._tensor("out", out, (None, None)).shape
-        self._mxfp4("x", xcodes, xscales, R, k)
-        self._mxfp4("w", wcodes, wscales, E * n, k)
+        if out.dim() != 2:
+            self._bad("out", out, "[R, n]")
+        (R, n), E = out.shape, seg_off.shape[0] - 1
+        self._vec("seg_off", seg_off, E + 1, torch.int32)
+        self._mxfp4("MXFP4 rows of x", xcodes, xscales, R, k)
+        self._mxfp4("MXFP4 rows of w", wcodes, wscales, E * n, k)
         self._check(lib().moe_grouped_mm_mxfp4(self._h, E, R, n, k, xcodes.data_ptr(),
                                                xscales.data_ptr(), wcodes.data_ptr(),
                                                wscales.data_ptr(), seg_off.data_ptr(),
-                                               out.data_ptr(), _dt(out), self._ld("out", out, n),
-                                               _stream(stream)))
+                                               out.data_ptr(), _dt(out),
+                                               self._rows("out", out, R, n), _op_stream(stream)))
 
-    def _norm_desc(self, res, blk, gains, gate, post_norm, residual_scale, eps):
-        """Shared checks: res / blk are the named [T, H] tensors of the residual
-        and the block (None where absent); the tensors of a kind share type and
-        row stride."""
+    def _norm_desc(self, res, blk, gains, gates, post_norm, residual_scale, eps):
+        """Shared checks: res and blk are the named [T, H] tensors of the residual
+        and of the block (None where absent); those of a kind share type and row
+        stride."""
         import torch
-        T, H = next(t for _, t in res if t is not None).shape
-        ld = []
+        T, H = shape = next(t for _, t in res if t is not None).shape
+        kinds = []
         for kind in (res, blk):
-            first = next(((s, t) for s, t in kind if t is not None), None)
-            for s, t in kind:
+            dtype = ld = None
+            for name, t in kind:
                 if t is None:
                     continue
-                self._tensor(s, t, (T, H), first[1].dtype)
-                if self._ld(s, t, H) != self._ld(first[0], first[1], H):
-                    raise MoeError(MOE_ERR_INVALID, f"{s} and {first[0]}: row strides differ")
-            ld.append(None if first is None else (_dt(first[1]), self._ld(*first, H)))
-        for s, t in gains:
-            if t is not None:
-                self._tensor(s, t, (H,), torch.float32)
-        for s, t in gate:
-            if t is not None and not self._tensor(s, t, (T,), torch.float32).is_contiguous():
-                raise MoeError(MOE_ERR_INVALID, f"{s} is not contiguous")
-        (rd, rld), (bd, bld) = ld[0], ld[1] or ld[0]
-        return MoeBlockNormDesc(T, H, rd, bd, rld, bld, int(post_norm), residual_scale, eps)
+                if dtype is None:
+                    dtype, ld = t.dtype, self._rows(name, t, T, H)
+                    kinds += _dt(t), ld
+                elif t.dtype != dtype or self._rows(name, t, T, H) != ld:
+                    self._bad(name, t, f"{dtype} rows {ld} apart, as {kind[0][0]}'s,")
+        for name, t in gains:
+            self._vec(name, t, H, torch.float32)
+        for name, t in gates:
+            self._vec(name, t, T, torch.float32)
+        rd, rld, bd, bld = kinds if len(kinds) == 4 else kinds * 2
+        return MoeBlockNormDesc(T, H, rd, bd, rld, bld, post_norm, residual_scale, eps)
 
     def block_norm(self, x, x_out, h, w_pre=None, y=None, w_post=None, gate=None,
                    post_norm: bool = True, residual_scale: float = 1.0, eps: float = 1e-5,
@@ -317,12 +353,12 @@ class MoeLayerEngine:
         w_pre (RMS norms; post_norm=False adds gate * y).  x, x_out [T, H] of one
         type; y, h [T, H] of that type, or of any when x is f32; gains f32 [H],
         gate f32 [T]; x_out or h may be None, x_out may be x and h may be y."""
-        d = self._norm_desc([("x", x), ("x_out", x_out)], [("y", y), ("h", h)],
-                            [("w_pre", w_pre), ("w_post", w_post)], [("gate", gate)], post_norm,
+        d = self._norm_desc((("x", x), ("x_out", x_out)), (("y", y), ("h", h)),
+                            (("w_pre", w_pre), ("w_post", w_post)), (("gate", gate),), post_norm,
                             residual_scale, eps)
         self._check(lib().moe_block_norm(self._h, d, x.data_ptr(), _ptr(y), _ptr(w_post),
                                          _ptr(gate), _ptr(w_pre), _ptr(x_out), _ptr(h),
-                                         _stream(stream)))
+                                         _op_stream(stream)))
 
     def block_norm_backward(self, dx_out, dh, x_out, w_pre, dx, dw_pre=None, y=None, w_post=None,
                             gate=None, dy=None, dw_post=None, dgate=None, post_norm: bool = True,
@@ -331,24 +367,24 @@ class MoeLayerEngine:
         given, the gradients of the gains (f32 [H]) and of the gate (f32 [T]).
         dx_out or dh may be None (zeros); dx may be dx_out and dy may be dh."""
         import torch
-        d = self._norm_desc([("x_out", x_out), ("dx_out", dx_out), ("dx", dx)],
-                            [("dh", dh), ("y", y), ("dy", dy)],
-                            [("w_pre", w_pre), ("w_post", w_post), ("dw_pre", dw_pre),
-                             ("dw_post", dw_post)], [("gate", gate), ("dgate", dgate)], post_norm,
+        d = self._norm_desc((("x_out", x_out), ("dx_out", dx_out), ("dx", dx)),
+                            (("dh", dh), ("y", y), ("dy", dy)),
+                            (("w_pre", w_pre), ("w_post", w_post), ("dw_pre", dw_pre),
+                             ("dw_post", dw_post)), (("gate", gate), ("dgate", dgate)), post_norm,
                             residual_scale, eps)
-        need = lib().moe_block_norm_backward_workspace(self._h, d.rows, d.hidden)
-        dev = torch.device("cuda", self.device)
-        if stream is None:
-            stream = torch.cuda.ExternalStream(lib().moe_get_stream(self._h), device=dev)
-        # from the pool of the stream that uses it, so that its reuse is ordered there
-        with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else
-                               torch.cuda.ExternalStream(stream, device=dev)):
-            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        self._check(lib().moe_block_norm_backward(self._h, d, _ptr(dx_out), _ptr(dh),
-                                                  x_out.data_ptr(), _ptr(y), _ptr(w_post),
-                                                  _ptr(gate), _ptr(w_pre), dx.data_ptr(), _ptr(dy),
-                                                  _ptr(dw_post), _ptr(dgate), _ptr(dw_pre),
-                                                  ws.data_ptr(), need, _stream(stream)))
+        L = lib()
+        need = L.moe_block_norm_backward_workspace(self._h, d.rows, d.hidden)
+        s = _op_stream(stream) or L.moe_get_stream(self._h)
+        if s == _op_stream(torch.cuda.current_stream(self._dev)):
+            ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+        else:  # from the pool of the stream that uses it: its reuse is ordered there
+            with torch.cuda.stream(torch.cuda.default_stream(self._dev) if s == 1 else
+                                   torch.cuda.ExternalStream(s, device=self._dev)):
+                ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+        self._check(L.moe_block_norm_backward(self._h, d, _ptr(dx_out), _ptr(dh), x_out.data_ptr(),
+                                              _ptr(y), _ptr(w_post), _ptr(gate), _ptr(w_pre),
+                                              dx.data_ptr(), _ptr(dy), _ptr(dw_post), _ptr(dgate),
+                                              _ptr(dw_pre), ws.data_ptr(), need, s))
 
     def set_wait_limit(self, ns: int = 0):
         """Bound of the device-side waits (grid barriers, expert-parallel flag

@@ -17,8 +17,10 @@ U = 2.0 ** -24
 @pytest.fixture(scope="module")
 def eng():
     e = M.MoeLayerEngine(M.MoeConfig(64, 32, 8, 2, True, 16, 1))
-    e.set_stream(torch.cuda.current_stream())
-    yield e
+    s = torch.cuda.Stream()
+    e.set_stream(s)
+    with torch.cuda.stream(s):  # the tests' own tensors are made on the handle's stream
+        yield e
     torch.cuda.synchronize()
     e.close()
 
@@ -700,7 +702,7 @@ def test_training_step_in_a_graph(eng):
 
 def test_two_streams_at_once(eng):
     """The same calls on two streams at the same time, without shared state."""
-    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    streams = [torch.cuda.Stream(), torch.cuda.default_stream()]
     T, H, n = 600, 256, 264
     off, _ = offsets([200, 0, 395, 5])
     ins = [dict(x=whole((T, H), BF, 30 + j), w=whole((4, n, H), BF, 40 + j)) for j in range(2)]
@@ -720,6 +722,27 @@ def test_two_streams_at_once(eng):
     for j in range(2):
         for key in ("o", "dw", "dx"):
             assert torch.equal(outs[0][j][key], outs[1][j][key])
+
+
+def test_default_stream_is_torchs(eng):
+    """torch's default stream, whose handle is 0, orders a call behind the work
+    that makes its inputs and before the work that reads its result."""
+    off, _ = offsets([100, 156])
+    w = whole((2, 64, 512), BF, 1)
+    with torch.cuda.stream(torch.cuda.default_stream()):
+        torch.cuda.synchronize()
+        a = torch.ones(4096, 4096, device="cuda")
+        for _ in range(4):  # some milliseconds of work in front
+            a = a @ a / 4096
+        x = (a[:256, :512] * 2).to(BF)
+        out = torch.zeros(256, 64, device="cuda")
+        eng.grouped_mm(x, w, off, out, stream=torch.cuda.current_stream())
+        got = out + 0
+        x.zero_()
+        torch.cuda.synchronize()
+    two = torch.full((256, 512), 2.0, dtype=torch.float64, device="cuda")
+    ref = torch.cat((two[:100] @ w[0].double().T, two[100:] @ w[1].double().T))
+    assert torch.equal(got, ref.float())
 
 
 def test_handle_stream_and_profile(eng):

@@ -6,6 +6,7 @@ import pytest
 
 import doantotnghiepmoe_b200 as M
 from doantotnghiepmoe_b200 import _lib
+from doantotnghiepmoe_b200.layer import mxfp4_strides
 
 
 def test_mxfp4_row_sizes():
@@ -14,6 +15,7 @@ def test_mxfp4_row_sizes():
                              (2048, 1024, 64), (0, 0, 0), (-5, 0, 0)):
         assert L.moe_mxfp4_code_stride(k) == codes
         assert L.moe_mxfp4_scale_stride(k) == scales
+        assert k < 1 or mxfp4_strides(k) == (codes, scales)
 
 
 def test_null_arguments_are_refused():
@@ -35,7 +37,7 @@ def test_null_arguments_are_refused():
 def test_host_tensors_are_refused():
     torch = pytest.importorskip("torch")
     eng = M.MoeLayerEngine.__new__(M.MoeLayerEngine)  # no handle: the checks come first
-    eng._h, eng.device = None, 0
+    eng._h, eng.device, eng._dev = None, 0, torch.device("cuda", 0)
     x, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(2, 8, 8, dtype=torch.bfloat16)
     off = torch.zeros(3, dtype=torch.int32)
     for call in (lambda: eng.grouped_mm(x, w, off, x), lambda: eng.grouped_mm_dgrad(x, w, off, x),
