@@ -52,16 +52,16 @@ struct Work {
   const GroupedArgs &a;
   const SegTable &seg;
   int nM, nN;
-  long long total;
+  int total;
   __device__ __forceinline__ Work(const GroupedArgs &a_, const SegTable &s) : a(a_), seg(s) {
     nM = ((KIND == kGroupedFwd ? a.n : a.k) + kTM - 1) / kTM;
     nN = (a.n + kTN - 1) / kTN;
-    total = KIND == kGroupedWgrad ? (long long)a.E * nM * nN : (long long)seg.total * nM;
+    total = KIND == kGroupedWgrad ? a.E * nM * nN : seg.total * nM;
   }
-  __device__ __forceinline__ Item item(long long w) const {
+  __device__ __forceinline__ Item item(int w) const {
     Item it;
-    it.m0 = (int)(w % nM) * kTM;
-    const int g = (int)(w / nM);
+    const int g = w / nM;
+    it.m0 = (w - g * nM) * kTM;
     if (KIND == kGroupedWgrad) {
       it.e = g / nN;
       it.c0 = g % nN * kTN;
@@ -100,43 +100,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after_sync();
   const Work<KIND> work(a, seg);
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     int q = 0;
-    for (long long w = blockIdx.x; w < work.total && !pp.abort_flag; w += gridDim.x) {
+    bool ok = true;
+    for (int w = blockIdx.x; w < work.total && ok; w += gridDim.x) {
       const Item it = work.item(w);
       const int nk = (it.len + kTK - 1) / kTK;
       const int nbox = kQMn ? (it.nc + 63) / 64 : (it.nc + kBoxRows - 1) / kBoxRows;
       const uint32_t bytes = kABytes + nbox * (kQMn ? kMnBox : kBoxRows * 128u);
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
-        if (use > 0 && !tma::mbar_wait(&pp.empty[s], (use - 1) & 1, &pp.abort_flag)) {
-          pp.abort_flag = 1;
-          break;
+        ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t *st = tiles + s * kStageBytes;
+          tma::mbar_expect_tx(&pp.full[s], bytes);
+          const int kr = it.row0 + kb * kTK;  // first row of K of an MN-major tile
+          if (kPMn) {
+            for (int i = 0; i < 2; ++i)
+              tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (it.m0 + 64 * i) * 2, kr,
+                           kQMn ? 0 : it.e);
+          } else {
+            tma::load_3d(st, &mapP, &pp.full[s], kb * 128, it.m0, it.e);
+          }
+          for (int i = 0; i < nbox; ++i) {
+            if (kQMn)
+              tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], (it.c0 + 64 * i) * 2, kr,
+                           0);
+            else
+              tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapQ, &pp.full[s], kb * 128,
+                           it.c0 + i * kBoxRows, 0);
+          }
         }
-        uint8_t *st = tiles + s * kStageBytes;
-        tma::mbar_expect_tx(&pp.full[s], bytes);
-        const int kr = it.row0 + kb * kTK;  // first row of K of an MN-major tile
-        if (kPMn) {
-          for (int i = 0; i < 2; ++i)
-            tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (it.m0 + 64 * i) * 2, kr,
-                         kQMn ? 0 : it.e);
-        } else {
-          tma::load_3d(st, &mapP, &pp.full[s], kb * 128, it.m0, it.e);
-        }
-        for (int i = 0; i < nbox; ++i) {
-          if (kQMn)
-            tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], (it.c0 + 64 * i) * 2, kr,
-                         0);
-          else
-            tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapQ, &pp.full[s], kb * 128,
-                         it.c0 + i * kBoxRows, 0);
-        }
+        __syncwarp();
       }
     }
-    if (pp.abort_flag) {  // issued stages must land before the CTA may exit
+    if (!ok) {  // issued stages must land before the CTA may exit
       const int from = *(volatile int *)&pp.consumed;
       for (int k = from; k < q; ++k)
-        tma::mbar_wait(&pp.full[k % kStages], (k / kStages) & 1, nullptr);
+        tma::mbar_wait(&pp.full[k % kStages], (k / kStages) & 1, nullptr, tma::kWaitCycles / 64);
     }
   } else if (warp == 1) {
     // fp32 sums, both operands of one type, M = 128
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)kPMn << 15) |
                             ((uint32_t)kQMn << 16) | ((uint32_t)(kTM >> 4) << 24);
     int q = 0, j = 0;
-    for (long long w = blockIdx.x; w < work.total; w += gridDim.x) {
+    for (int w = blockIdx.x; w < work.total; w += gridDim.x) {
       const Item it = work.item(w);
       const int nk = (it.len + kTK - 1) / kTK;
       if (nk == 0) continue;
@@ -175,14 +177,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         fence_after_sync();
-        if (lane == 0) {
+        if (elect_one()) {
           const uint32_t base = su32(st);
-          for (int k = 0; k < steps; ++k) {
-            const uint64_t pd = kPMn ? sw128_desc(base + k * 2048, kMnBox, 1024)
-                                     : sw128_desc(base + k * 32, 16, 1024);
-            const uint64_t qd = kQMn ? sw128_desc(base + kABytes + k * 2048, kMnBox, 1024)
-                                     : sw128_desc(base + kABytes + k * 32, 16, 1024);
-            mma_f16(d, pd, qd, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          const uint64_t pd = kPMn ? sw128_desc(base, kMnBox, 1024) : sw128_desc(base, 16, 1024);
+          const uint64_t qd = kQMn ? sw128_desc(base + kABytes, kMnBox, 1024)
+                                   : sw128_desc(base + kABytes, 16, 1024);
+          // 16 elements of K further: 32 bytes of a row, or 16 rows of 128 bytes
+          constexpr uint64_t kPStep = (kPMn ? 2048 : 32) >> 4, kQStep = (kQMn ? 2048 : 32) >> 4;
+          if (steps == kTK / 16) {
+#pragma unroll
+            for (int k = 0; k < kTK / 16; ++k)
+              mma_f16(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          } else {
+            for (int k = 0; k < steps; ++k)
+              mma_f16(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
           }
           commit(&pp.empty[s]);
           pp.consumed = q + 1;
@@ -190,16 +198,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
       if (!ok) break;
-      if (lane == 0) commit(&pp.tfull[buf]);
+      if (elect_one()) commit(&pp.tfull[buf]);
       ++j;
     }
-    if (lane == 0) commit(&pp.done);
+    if (elect_one()) commit(&pp.done);
   } else if (warp >= 2) {
     const int quarter = warp & 3, grp = (warp - 2) >> 2;
     const int M = KIND == kGroupedFwd ? a.n : a.k;
     const int64_t ld = KIND == kGroupedFwd ? a.ld_out : KIND == kGroupedDgrad ? a.ld_x : a.ld_w;
     int j = 0;
-    for (long long w = blockIdx.x; w < work.total; w += gridDim.x) {
+    for (int w = blockIdx.x; w < work.total; w += gridDim.x) {
       const Item it = work.item(w);
       const int m = it.m0 + quarter * 32 + lane;
       const int64_t at0 = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
@@ -236,6 +244,7 @@ cudaError_t launch_kind(const CUtensorMap &p, const CUtensorMap &q, const Groupe
   const long long nM = ((KIND == kGroupedFwd ? a.n : a.k) + kTM - 1) / kTM;
   const long long g = KIND == kGroupedWgrad ? (long long)a.E * ((a.n + kTN - 1) / kTN)
                                             : a.R / kTN + std::min(a.E, a.R);
+  if (g * nM > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
   const int grid = (int)std::min<long long>(g * nM, a.sm_count);
   grouped_tc_kernel<KIND><<<grid, kThreads, kSmem, s>>>(p, q, a);
   return cudaGetLastError();

@@ -63,14 +63,14 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   fence_after_sync();
 
   const int nM = (a.n + kTM - 1) / kTM, nk = (a.k + 255) / 256;
-  const long long total = (long long)seg.total * nM;
+  const int total = seg.total * nM;
   struct Item {
     int e, m0, c0, nc;
   };
-  const auto item = [&](long long w) {
+  const auto item = [&](int w) {
     Item it;
-    it.m0 = (int)(w % nM) * kTM;
-    const int g = (int)(w / nM);
+    const int g = w / nM;
+    it.m0 = (w - g * nM) * kTM;
     it.e = seg.expert_of(g, a.E);
     const int cnt = seg.rows(it.e), nt = seg.tile0[it.e + 1] - seg.tile0[it.e];
     const int sz = tile_rows(cnt, nt), t = g - seg.tile0[it.e];
@@ -79,26 +79,28 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     return it;
   };
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     int q = 0;
-    for (long long w = blockIdx.x; w < total && !pp.abort_flag; w += gridDim.x) {
+    bool ok = true;
+    for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
       const Item it = item(w);
       const int nbox = (it.nc + kBoxRows - 1) / kBoxRows;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
-        if (use > 0 && !tma::mbar_wait(&pp.empty[s], (use - 1) & 1, &pp.abort_flag)) {
-          pp.abort_flag = 1;
-          break;
+        ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t *st = tiles + s * kStageBytes;
+          tma::mbar_expect_tx(&pp.full[s], kABytes + nbox * kBoxRows * 128u);
+          tma::load_3d(st, &mapW, &pp.full[s], kb * 128, it.m0, it.e);
+          for (int i = 0; i < nbox; ++i)
+            tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapX, &pp.full[s], kb * 128,
+                         it.c0 + i * kBoxRows, 0);
         }
-        uint8_t *st = tiles + s * kStageBytes;
-        tma::mbar_expect_tx(&pp.full[s], kABytes + nbox * kBoxRows * 128u);
-        tma::load_3d(st, &mapW, &pp.full[s], kb * 128, it.m0, it.e);
-        for (int i = 0; i < nbox; ++i)
-          tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapX, &pp.full[s], kb * 128,
-                       it.c0 + i * kBoxRows, 0);
+        __syncwarp();
       }
     }
-    if (pp.abort_flag) {  // issued stages must land before the CTA may exit
+    if (!ok) {  // issued stages must land before the CTA may exit
       const int from = *(volatile int *)&pp.consumed;
       for (int k = from; k < q; ++k)
         tma::mbar_wait(&pp.full[k % kStages], (k / kStages) & 1, nullptr, tma::kWaitCycles / 64);
@@ -108,14 +110,13 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kTM >> 4) << 24);
     const uint32_t sf0 = pp.tmem_base + 2 * kTN;
     int q = 0, j = 0;
-    for (long long w = blockIdx.x; w < total; w += gridDim.x, ++j) {
+    for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
       const int buf = j & 1;
       if (j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
       fence_after_sync();
       const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 15) >> 4) << 18);
-      const int rgroups = (it.nc + 127) / 128;
       bool ok = true;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages;
@@ -129,22 +130,22 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           break;
         }
         fence_after_sync();
-        if (lane == 0) {
+        if (elect_one()) {
           const uint32_t base = su32(tiles + s * kStageBytes);
-          const uint32_t sb = su32(scales + s * kScaleBytes);
+          const uint64_t sd = rows16_desc(su32(scales + s * kScaleBytes));
+          const uint64_t wd = sw128_desc(base, 16, 1024), xd = sw128_desc(base + kABytes, 16, 1024);
           const uint32_t sfa = sf0 + (uint32_t)(q % kSets) * kSetCols, sfb = sfa + 8;
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            cp_scales(sfa + 4 * g, rows16_desc(sb + g * kGroup));
-            for (int r = 0; r < rgroups; ++r)
-              cp_scales(sfb + 8 * g + 4 * r, rows16_desc(sb + (2 + 2 * g + r) * kGroup));
+            cp_scales(sfa + 4 * g, sd + (g * kGroup >> 4));
+            cp_scales(sfb + 8 * g, sd + ((2 + 2 * g) * kGroup >> 4));
+            if (it.nc > 128) cp_scales(sfb + 8 * g + 4, sd + ((3 + 2 * g) * kGroup >> 4));
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = (uint32_t)(k & 1) * 2;  // bytes 0-1 or 2-3 of a scale word
-            mma_mxf4(d, sw128_desc(base + k * 32, 16, 1024),
-                     sw128_desc(base + kABytes + k * 32, 16, 1024), idesc | (id << 4) | (id << 29),
-                     sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
+            mma_mxf4(d, wd + 2 * k, xd + 2 * k, idesc | (id << 4) | (id << 29), sfa + 4 * (k >> 1),
+                     sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
           }
           commit(&pp.empty[s]);
           pp.consumed = q + 1;
@@ -152,14 +153,14 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         __syncwarp();
       }
       if (!ok) break;
-      if (lane == 0) commit(&pp.tfull[buf]);
+      if (elect_one()) commit(&pp.tfull[buf]);
     }
-    if (lane == 0) commit(&pp.done);
+    if (elect_one()) commit(&pp.done);
   } else if (warp >= 2 && warp < 2 + kScaleWarps) {
     const int words = mxfp4_scale_stride(a.k) / 4;
     const uint32_t *xs = reinterpret_cast<const uint32_t *>(a.xs);
     const uint32_t *ws = reinterpret_cast<const uint32_t *>(a.ws);
-    long long w = blockIdx.x;
+    int w = blockIdx.x;
     int kb = warp - 2;  // this warp's steps: every kScaleWarps-th
     for (int q = warp - 2;; q += kScaleWarps, kb += kScaleWarps) {
       for (; kb >= nk && w < total; kb -= nk) w += gridDim.x;
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   } else if (warp >= 2) {
     const int ew = warp - 2 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
     int j = 0;
-    for (long long w = blockIdx.x; w < total; w += gridDim.x, ++j) {
+    for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
       const int m = it.m0 + quarter * 32 + lane, buf = j & 1;
       if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
@@ -224,6 +225,7 @@ cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
       !tc::encode_map3d(&x, a.xc, row, (uint64_t)a.R, 1, row, row, kBoxRows))
     return cudaErrorInvalidValue;
   const long long items = (long long)(a.R / kTN + std::min(a.E, a.R)) * ((a.n + kTM - 1) / kTM);
+  if (items > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
   mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(w, x, a);
   return cudaGetLastError();
 }
