@@ -38,7 +38,8 @@ constexpr uint32_t kABytes = kTM * 128, kStageBytes = (kTM + kTN) * 128;
 constexpr int kBoxRows = 32;                 // N-side rows of one copy (K-major)
 constexpr uint32_t kMnBox = kTK * 128;       // one copy of an MN-major side: 64 of M or N
 constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
-                         (size_t)kStages * kStageBytes;
+                         (size_t)kStages * kStageBytes + kEpiWarps * kDrainBytes;
+static_assert(kSmem <= 232448, "shared memory");
 
 struct Item {
   int e, m0;  // expert, first M index
@@ -135,11 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     }
-    if (!ok) {  // issued stages must land before the CTA may exit
-      const int from = *(volatile int *)&pp.consumed;
-      for (int k = from; k < q; ++k)
-        tma::mbar_wait(&pp.full[k % kStages], (k / kStages) & 1, nullptr, tma::kWaitCycles / 64);
-    }
+    if (!ok) pp.drain(q);
   } else if (warp == 1) {
     // fp32 sums, both operands of one type, M = 128
     const uint32_t fmt = a.dtype == MOE_DT_BF16 ? 1u : 0u;
@@ -193,7 +190,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               mma_f16(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
           }
           commit(&pp.empty[s]);
-          pp.consumed = q + 1;
         }
         __syncwarp();
       }
@@ -204,13 +200,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect_one()) commit(&pp.done);
   } else if (warp >= 2) {
     const int quarter = warp & 3, grp = (warp - 2) >> 2;
+    uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kStages * kStageBytes +
+                                                   (warp - 2) * kDrainBytes);
     const int M = KIND == kGroupedFwd ? a.n : a.k;
     const int64_t ld = KIND == kGroupedFwd ? a.ld_out : KIND == kGroupedDgrad ? a.ld_x : a.ld_w;
     int j = 0;
     for (int w = blockIdx.x; w < work.total; w += gridDim.x) {
       const Item it = work.item(w);
-      const int m = it.m0 + quarter * 32 + lane;
-      const int64_t at0 = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
+      const int m = it.m0 + quarter * 32;
+      const int64_t at = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
       const bool some = it.len > 0;
       const int buf = j & 1;
       if (some) {
@@ -220,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint32_t trow =
           pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16);
-      drain_tile(trow, some, it.nc, grp, m < M, a.out, a.out_dtype, at0, ld);
+      drain_tile(trow, some, it.nc, grp, M - m, a.out, a.out_dtype, at, ld, buf32);
       if (some) {
         fence_before_sync();
         __syncwarp();

@@ -13,9 +13,9 @@
 // blocks (128 elements of K), in the order of the rows' lanes.  Scale bytes
 // lie by row in memory; four warps, each at another stage, fetch 4 of them at
 // a time and store them in the order that a 32-row copy to TMEM takes: word
-// (r % 32) * 4 + r / 32 of a 512-byte group.  192 rows of N rather than 256 leave room in TMEM for four
-// sets of scales beside the two buffers, so that a set is written again only
-// after the MMAs that read it are known to be done.
+// (r % 32) * 4 + r / 32 of a 512-byte group.  192 rows of N rather than 256 leave room in TMEM for a
+// set of scales a stage beside the two buffers: a stage is filled again only
+// once its MMAs are done, and so its set is free with it.
 #include <cuda.h>
 
 #include <algorithm>
@@ -31,18 +31,18 @@ namespace {
 using namespace tcp;
 
 constexpr int kTM = 128, kTN = 192;
-constexpr int kStages = 5, kSets = 4;
+constexpr int kStages = 4;
 constexpr uint32_t kABytes = kTM * 128, kBBytes = kTN * 128, kStageBytes = kABytes + kBBytes;
 constexpr int kBoxRows = 32;
 constexpr int kGroup = 512;            // scale bytes of 128 rows and 4 blocks
 constexpr int kScaleBytes = 6 * kGroup;  // of a stage: 2 groups of w, 2 x 2 of x
 constexpr int kSetCols = 24;             // TMEM columns of a stage's scales
 constexpr uint32_t kTmemCols = 512;
-static_assert(2 * kTN + kSets * kSetCols <= (int)kTmemCols, "TMEM");
+static_assert(2 * kTN + kStages * kSetCols <= (int)kTmemCols, "TMEM");
 constexpr int kScaleWarps = 4;
 constexpr int kMxThreads = kThreads + 32 * kScaleWarps;
 constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
-                         (size_t)kStages * (kStageBytes + kScaleBytes);
+                         (size_t)kStages * (kStageBytes + kScaleBytes) + kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
 
 __global__ void __launch_bounds__(kMxThreads, 1)
@@ -100,11 +100,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         __syncwarp();
       }
     }
-    if (!ok) {  // issued stages must land before the CTA may exit
-      const int from = *(volatile int *)&pp.consumed;
-      for (int k = from; k < q; ++k)
-        tma::mbar_wait(&pp.full[k % kStages], (k / kStages) & 1, nullptr, tma::kWaitCycles / 64);
-    }
+    if (!ok) pp.drain(q);
   } else if (warp == 1) {
     // E2M1 operands, E8M0 scales, M = 128
     const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kTM >> 4) << 24);
@@ -120,12 +116,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       bool ok = true;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages;
-        // the MMAs that read this set of scales are done
-        if (q >= kSets) {
-          const int p = q - kSets;
-          ok = pp.wait_warp(&pp.empty[p % kStages], (p / kStages) & 1);
-        }
-        if (!ok || !pp.wait_warp(&pp.full[s], (q / kStages) & 1)) {
+        if (!pp.wait_warp(&pp.full[s], (q / kStages) & 1)) {
           ok = false;
           break;
         }
@@ -134,7 +125,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           const uint32_t base = su32(tiles + s * kStageBytes);
           const uint64_t sd = rows16_desc(su32(scales + s * kScaleBytes));
           const uint64_t wd = sw128_desc(base, 16, 1024), xd = sw128_desc(base + kABytes, 16, 1024);
-          const uint32_t sfa = sf0 + (uint32_t)(q % kSets) * kSetCols, sfb = sfa + 8;
+          const uint32_t sfa = sf0 + (uint32_t)s * kSetCols, sfb = sfa + 8;
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             cp_scales(sfa + 4 * g, sd + (g * kGroup >> 4));
@@ -148,7 +139,6 @@ __global__ void __launch_bounds__(kMxThreads, 1)
                      sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
           }
           commit(&pp.empty[s]);
-          pp.consumed = q + 1;
         }
         __syncwarp();
       }
@@ -192,14 +182,16 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     }
   } else if (warp >= 2) {
     const int ew = warp - 2 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
+    uint32_t *buf32 = reinterpret_cast<uint32_t *>(scales + kStages * kScaleBytes +
+                                                   ew * kDrainBytes);
     int j = 0;
     for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
-      const int m = it.m0 + quarter * 32 + lane, buf = j & 1;
+      const int m = it.m0 + quarter * 32, buf = j & 1;
       if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
       fence_after_sync();
       drain_tile(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), true,
-                 it.nc, grp, m < a.n, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out);
+                 it.nc, grp, a.n - m, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out, buf32);
       fence_before_sync();
       __syncwarp();
       if (lane == 0) tma::mbar_arrive(&pp.tempty[buf]);

@@ -120,7 +120,6 @@ struct Pipe {
   uint64_t done;                 // every MMA of this CTA has completed
   uint32_t tmem_base;
   int abort_flag;
-  int consumed;  // stages that the issuing warp has taken
 
   __device__ __forceinline__ void init(uint32_t full_count) {
     for (int s = 0; s < S; ++s) {
@@ -133,11 +132,17 @@ struct Pipe {
     }
     tma::mbar_init(&done, 1);
     abort_flag = 0;
-    consumed = 0;
     tma::fence_mbar_init();
+  }
+  // After q issued stages and an abort: the copies in flight land before the
+  // CTA may exit (a bounded wait for the last use of each stage).
+  __device__ __forceinline__ void drain(int q) {
+    for (int k = max(q - S, 0); k < q; ++k)
+      tma::mbar_wait(&full[k % S], (k / S) & 1, nullptr, tma::kWaitCycles / 64);
   }
   // A whole warp's bounded wait; false (for every lane) once any role gave up.
   __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, tma::mbar_try(bar, parity))) return true;  // the usual case
     const bool ok = tma::mbar_wait(bar, parity, &abort_flag);
     if (__all_sync(0xffffffffu, ok)) return true;
     abort_flag = 1;
@@ -149,18 +154,101 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
   return reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
 }
 
-// Writes a tile's sums: column c of the accumulator is row c of the result,
-// and lane l of a quarter its element m0 + l.  Called by the 8 draining warps,
-// grp the half of the columns (in turns of 32) that this warp takes.
-template <typename T>
-__device__ __forceinline__ void store_cols(T *out, int64_t ld, int c, int nc,
-                                           const uint32_t (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (c + i < nc) out[(c + i) * ld] = from_f32<T>(__uint_as_float(v[i]));
+// The epilogue of a tile: column c of the accumulator is row c of the result,
+// and lane l of a quarter its element m + l.  A warp's 32 lanes would store 64
+// bytes of a 16-bit row at a time (measured: 14 cycles a store, the bound of
+// wgrad), so 32 columns (16 of an fp32 result) go through 2 KB of shared memory
+// of the warp's own and leave as 16 bytes a lane, whole sectors of 8 rows (4) a
+// store.  16-bit values go as pairs of columns, one word a lane, and are parted
+// on the way out.
+constexpr int kDrainBytes = 2048;  // of shared memory, for each draining warp
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
 }
-__device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int grp, bool inside,
-                                           void *out, int out_dtype, int64_t at, int64_t ld) {
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// 8 (4 of fp32) elements of a row, of which the first `left` are inside it.
+template <typename T>
+__device__ __forceinline__ void store_piece(T *p, uint4 v, int left) {
+  constexpr int kN = 16 / sizeof(T);
+  if (left >= kN) {
+    *reinterpret_cast<uint4 *>(p) = v;
+  } else {
+    const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (i < left) p[i] = e[i];
+  }
+}
+
+// Columns c .. c + 31 of the accumulator (v), row c of the result at out; the
+// warp's elements of a row start at out and `left` of its 32 are inside.
+template <typename T>
+__device__ __forceinline__ void store_cols(T *out, int64_t ld, int nc, int left, bool vec,
+                                           uint32_t *buf, const uint32_t (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  if (!vec) {  // rows that do not start on 16 bytes: a lane's own element of each
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < nc && lane < left) out[i * ld + lane] = from_f32<T>(__uint_as_float(v[i]));
+    __syncwarp();
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int p = 0; p < 16; ++p)
+      buf[p * 32 + lane] =
+          pack2(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]), T{});
+    __syncwarp();
+    const int m = lane % 4 * 8;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int p = lane / 4 + 8 * t;
+      const uint4 a = *reinterpret_cast<const uint4 *>(buf + p * 32 + m);
+      const uint4 b = *reinterpret_cast<const uint4 *>(buf + p * 32 + m + 4);
+      T *row = out + 2 * p * ld + m;
+      if (2 * p < nc)
+        store_piece(row, make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                                    __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410)),
+                    left - m);
+      if (2 * p + 1 < nc)
+        store_piece(row + ld,
+                    make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                               __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632)),
+                    left - m);
+    }
+    __syncwarp();
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) buf[i * 32 + lane] = v[16 * h + i];
+      __syncwarp();
+      const int m = lane % 8 * 4;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = lane / 8 + 4 * t;
+        if (16 * h + i < nc)
+          store_piece(out + (16 * h + i) * ld + m,
+                      *reinterpret_cast<const uint4 *>(buf + i * 32 + m), left - m);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// out: element (row 0, m0 + 32 quarter) of the tile as a byte pointer; grp the
+// half of the columns (in turns of 32) that this warp takes.
+__device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int grp, int left,
+                                           void *out, int out_dtype, int64_t at, int64_t ld,
+                                           uint32_t *buf) {
+  const int size = out_dtype == MOE_DT_F32 ? 4 : 2;
+  const bool vec = (((uintptr_t)out + at * size) & 15) == 0 && ((ld * size) & 15) == 0;
   for (int c = grp * 32; c < nc; c += 64) {
     uint32_t v[32];
     if (some) {
@@ -170,13 +258,13 @@ __device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = 0;
     }
-    if (inside) {
-      if (out_dtype == MOE_DT_F32) store_cols(reinterpret_cast<float *>(out) + at, ld, c, nc, v);
-      else if (out_dtype == MOE_DT_BF16)
-        store_cols(reinterpret_cast<__nv_bfloat16 *>(out) + at, ld, c, nc, v);
-      else store_cols(reinterpret_cast<__half *>(out) + at, ld, c, nc, v);
-    }
-    __syncwarp();  // the next load is the whole warp's
+    if (out_dtype == MOE_DT_F32)
+      store_cols(reinterpret_cast<float *>(out) + at + c * ld, ld, nc - c, left, vec, buf, v);
+    else if (out_dtype == MOE_DT_BF16)
+      store_cols(reinterpret_cast<__nv_bfloat16 *>(out) + at + c * ld, ld, nc - c, left, vec, buf,
+                 v);
+    else
+      store_cols(reinterpret_cast<__half *>(out) + at + c * ld, ld, nc - c, left, vec, buf, v);
   }
 }
 
