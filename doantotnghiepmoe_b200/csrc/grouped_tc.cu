@@ -13,7 +13,7 @@
 // One persistent CTA an SM walks the items (128 of M x up to 256 of N): one
 // thread keeps a ring of 4 stages (48 KB: 64 elements of K of both sides) full
 // by TMA across items, one warp issues the MMAs into two accumulator buffers
-// of 256 TMEM columns, and 8 warps drain one while the other fills.  Tiles
+// of 256 TMEM columns, and 16 warps drain one while the other fills.  Tiles
 // that reach past a segment read other experts' rows and drop their columns;
 // in wgrad, where the rows are summed, the rows of the last K step that belong
 // to others are zeroed in shared memory before the MMA (zeros alone would not

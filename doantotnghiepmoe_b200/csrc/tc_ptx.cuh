@@ -110,7 +110,8 @@ __device__ __forceinline__ uint64_t rows16_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 
-constexpr int kEpiWarps = 8;                   // two a TMEM lane quarter
+
+constexpr int kEpiWarps = 16;                  // four a TMEM lane quarter
 constexpr int kThreads = 64 + 32 * kEpiWarps;  // and the copying and issuing warps
 
 template <int S>
@@ -157,11 +158,11 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
 // The epilogue of a tile: column c of the accumulator is row c of the result,
 // and lane l of a quarter its element m + l.  A warp's 32 lanes would store 64
 // bytes of a 16-bit row at a time (measured: 14 cycles a store, the bound of
-// wgrad), so 32 columns (16 of an fp32 result) go through 2 KB of shared memory
-// of the warp's own and leave as 16 bytes a lane, whole sectors of 8 rows (4) a
-// store.  16-bit values go as pairs of columns, one word a lane, and are parted
-// on the way out.
-constexpr int kDrainBytes = 2048;  // of shared memory, for each draining warp
+// wgrad), so 16 columns (8 of an fp32 result) at a time go through 1 KB of shared
+// memory of the warp's own and leave as 16 bytes a lane, whole sectors of 8
+// rows (4) a store.  16-bit values go as pairs of columns, one word a lane, and
+// are parted on the way out.
+constexpr int kDrainBytes = 1024;  // of shared memory, for each draining warp
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -200,56 +201,58 @@ __device__ __forceinline__ void store_cols(T *out, int64_t ld, int nc, int left,
     return;
   }
   if constexpr (sizeof(T) == 2) {
+    const int p = lane / 4, m = lane % 4 * 8;
 #pragma unroll
-    for (int p = 0; p < 16; ++p)
-      buf[p * 32 + lane] =
-          pack2(__uint_as_float(v[2 * p]), __uint_as_float(v[2 * p + 1]), T{});
-    __syncwarp();
-    const int m = lane % 4 * 8;
+    for (int h = 0; h < 2; ++h) {
+      if (16 * h >= nc) break;  // warp-uniform
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int p = lane / 4 + 8 * t;
+      for (int i = 0; i < 8; ++i)
+        buf[i * 32 + lane] = pack2(__uint_as_float(v[16 * h + 2 * i]),
+                                   __uint_as_float(v[16 * h + 2 * i + 1]), T{});
+      __syncwarp();
       const uint4 a = *reinterpret_cast<const uint4 *>(buf + p * 32 + m);
       const uint4 b = *reinterpret_cast<const uint4 *>(buf + p * 32 + m + 4);
-      T *row = out + 2 * p * ld + m;
-      if (2 * p < nc)
+      const int i = 16 * h + 2 * p;
+      T *row = out + i * ld + m;
+      if (i < nc)
         store_piece(row, make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
                                     __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410)),
                     left - m);
-      if (2 * p + 1 < nc)
+      if (i + 1 < nc)
         store_piece(row + ld,
                     make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
                                __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632)),
                     left - m);
-    }
-    __syncwarp();
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) buf[i * 32 + lane] = v[16 * h + i];
       __syncwarp();
-      const int m = lane % 8 * 4;
+    }
+  } else {
+    const int m = lane % 8 * 4;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int i = lane / 8 + 4 * t;
-        if (16 * h + i < nc)
-          store_piece(out + (16 * h + i) * ld + m,
-                      *reinterpret_cast<const uint4 *>(buf + i * 32 + m), left - m);
+    for (int h = 0; h < 4; ++h) {
+      if (8 * h >= nc) break;  // warp-uniform
+#pragma unroll
+      for (int i = 0; i < 8; ++i) buf[i * 32 + lane] = v[8 * h + i];
+      __syncwarp();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = lane / 8 + 4 * t, i = 8 * h + r;
+        if (i < nc)
+          store_piece(out + i * ld + m, *reinterpret_cast<const uint4 *>(buf + r * 32 + m),
+                      left - m);
       }
       __syncwarp();
     }
   }
 }
 
-// out: element (row 0, m0 + 32 quarter) of the tile as a byte pointer; grp the
-// half of the columns (in turns of 32) that this warp takes.
+// at: the offset of the tile's element (row 0, m0 + 32 quarter); the groups of
+// four warps take the columns in turns of 32.
 __device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int grp, int left,
                                            void *out, int out_dtype, int64_t at, int64_t ld,
                                            uint32_t *buf) {
   const int size = out_dtype == MOE_DT_F32 ? 4 : 2;
   const bool vec = (((uintptr_t)out + at * size) & 15) == 0 && ((ld * size) & 15) == 0;
-  for (int c = grp * 32; c < nc; c += 64) {
+  for (int c = grp * 32; c < nc; c += kEpiWarps / 4 * 32) {
     uint32_t v[32];
     if (some) {
       tmem_ld32(trow + c, v);
