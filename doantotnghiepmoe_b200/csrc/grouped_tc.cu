@@ -10,14 +10,20 @@
 // first two, where an MMA may be any multiple of 16 wide, so a tile costs what
 // its rows are and not a full 128 (a decoded token pays 16 columns).
 //
-// One persistent CTA an SM walks the items (128 of M x up to 256 of N): one
-// thread keeps a ring of 4 stages (48 KB: 64 elements of K of both sides) full
-// by TMA across items, one warp issues the MMAs into two accumulator buffers
-// of 256 TMEM columns, and 16 warps drain one while the other fills.  Tiles
-// that reach past a segment read other experts' rows and drop their columns;
-// in wgrad, where the rows are summed, the rows of the last K step that belong
-// to others are zeroed in shared memory before the MMA (zeros alone would not
-// do on one side: 0 x NaN).  Every wait is bounded, as in expert_tc.cu.
+// A pair of CTAs (cta_group::2) works on one tile of 256 of M x up to 256 of N:
+// each CTA loads its 128 of M and half of the N side and keeps 128 rows of D.
+// Against a CTA's own 128 x 256 tile this moves 32 KB rather than 48 KB from L2
+// for the same products, and L2 to SM traffic is what bounded that kernel (54
+// bytes a cycle and SM).  One persistent CTA an SM: a warp keeps a ring of 6
+// stages (64 elements of K of both sides) full by TMA across items, the even
+// CTA's second warp issues the pair's MMAs into two accumulator buffers of 256
+// TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
+// odd CTA's second warp passes on that its stage has landed.  Tiles that reach
+// past a segment read other experts' rows and drop their columns; in wgrad,
+// where the rows are summed, the rows of the last K step that belong to others
+// are zeroed in shared memory before the MMA (zeros alone would not do on one
+// side: 0 x NaN).  Every wait on a barrier in memory is bounded, as in
+// expert_tc.cu.
 #include <cuda.h>
 
 #include <algorithm>
@@ -32,11 +38,11 @@ namespace {
 
 using namespace tcp;
 
-constexpr int kTM = 128, kTN = 256, kTK = 64;  // tile; kTK elements are 128 bytes
-constexpr int kStages = 4;
-constexpr uint32_t kABytes = kTM * 128, kStageBytes = (kTM + kTN) * 128;
-constexpr int kBoxRows = 32;                 // N-side rows of one copy (K-major)
-constexpr uint32_t kMnBox = kTK * 128;       // one copy of an MN-major side: 64 of M or N
+constexpr int kTM = 256, kTN = 256, kTK = 64;  // tile of a pair; kTK elements are 128 bytes
+constexpr int kStages = 6;
+constexpr uint32_t kABytes = kTM / 2 * 128, kStageBytes = (kTM + kTN) / 2 * 128;  // of a CTA
+constexpr int kBig = 64, kSmall = 16;     // N-side rows of one copy (K-major)
+constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
                          (size_t)kStages * kStageBytes + kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
@@ -72,7 +78,7 @@ struct Work {
     } else {
       it.e = seg.expert_of(g, a.E);
       const int cnt = seg.rows(it.e), nt = seg.tile0[it.e + 1] - seg.tile0[it.e];
-      const int sz = tile_rows(cnt, nt), t = g - seg.tile0[it.e];
+      const int sz = tile_rows<32>(cnt, nt), t = g - seg.tile0[it.e];
       it.c0 = seg.off[it.e] + t * sz;
       it.nc = min(sz, cnt - t * sz);
       it.row0 = 0;
@@ -82,10 +88,23 @@ struct Work {
   }
 };
 
+// Zeroes K rows [left, to) of the `boxes` MN-major copies of a stage.
+__device__ __forceinline__ void zero_rows(uint8_t *st, int boxes, int left, int to) {
+  const int lane = threadIdx.x & 31;
+  for (int r = left; r < to; ++r)
+    for (int i = lane; i < boxes * 8; i += 32)
+      *reinterpret_cast<uint4 *>(st + i / 8 * kMnBox + r * 128 + i % 8 * 16) =
+          make_uint4(0, 0, 0, 0);
+  tma::fence_proxy_async_smem();
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");  // the other CTA's thread issues the MMA
+  __syncwarp();
+}
+
 template <int KIND>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap mapP,
-                      const __grid_constant__ CUtensorMap mapQ, GroupedArgs a) {
+                      const __grid_constant__ CUtensorMap mapQ,
+                      const __grid_constant__ CUtensorMap mapQ16, GroupedArgs a) {
   constexpr bool kPMn = KIND != kGroupedFwd, kQMn = KIND == kGroupedWgrad;
   extern __shared__ uint8_t smem_raw[];
   using P = Pipe<kStages>;
@@ -93,22 +112,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   SegTable &seg = *reinterpret_cast<SegTable *>(smem_raw + sizeof(P));
   uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) pp.init(1);
-  if (warp == 1) tmem_alloc(&pp.tmem_base, 2 * kTN);
+  const int rank = (int)cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  // full: the even CTA's also counts the odd one's stage; tempty: both CTAs drain
+  if (threadIdx.x == 0) pp.init(rank == 0 ? 2 : 1, 2 * kEpiWarps);
+  if (warp == 1) tmem_alloc_pair(&pp.tmem_base, 2 * kTN);
   if (warp == 2) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
   fence_before_sync();
   __syncthreads();
+  cluster_sync();
   fence_after_sync();
   const Work<KIND> work(a, seg);
 
   if (warp == 0) {
     int q = 0;
     bool ok = true;
-    for (int w = blockIdx.x; w < work.total && ok; w += gridDim.x) {
+    for (int w = pair; w < work.total && ok; w += pairs) {
       const Item it = work.item(w);
       const int nk = (it.len + kTK - 1) / kTK;
-      const int nbox = kQMn ? (it.nc + 63) / 64 : (it.nc + kBoxRows - 1) / kBoxRows;
-      const uint32_t bytes = kABytes + nbox * (kQMn ? kMnBox : kBoxRows * 128u);
+      const int half = (it.nc + 31) / 32 * 16, c0 = it.c0 + rank * half, m0 = it.m0 + rank * 128;
+      const int nbig = kQMn ? (half + 63) / 64 : half / kBig;
+      const int nsmall = kQMn ? 0 : half % kBig / kSmall;
+      const uint32_t bytes = kABytes + nbig * kMnBox + nsmall * kSmall * 128u;
+      static_assert(kBig * 128 == kMnBox, "one box size");
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
         ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
@@ -119,39 +145,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int kr = it.row0 + kb * kTK;  // first row of K of an MN-major tile
           if (kPMn) {
             for (int i = 0; i < 2; ++i)
-              tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (it.m0 + 64 * i) * 2, kr,
+              tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (m0 + 64 * i) * 2, kr,
                            kQMn ? 0 : it.e);
           } else {
-            tma::load_3d(st, &mapP, &pp.full[s], kb * 128, it.m0, it.e);
+            tma::load_3d(st, &mapP, &pp.full[s], kb * 128, m0, it.e);
           }
-          for (int i = 0; i < nbox; ++i) {
+          for (int i = 0; i < nbig; ++i) {
             if (kQMn)
-              tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], (it.c0 + 64 * i) * 2, kr,
-                           0);
+              tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], (c0 + 64 * i) * 2, kr, 0);
             else
-              tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapQ, &pp.full[s], kb * 128,
-                           it.c0 + i * kBoxRows, 0);
+              tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], kb * 128,
+                           c0 + i * kBig, 0);
           }
+          for (int i = 0; i < nsmall; ++i)
+            tma::load_3d(st + kABytes + nbig * kMnBox + i * kSmall * 128, &mapQ16, &pp.full[s],
+                         kb * 128, c0 + nbig * kBig + i * kSmall, 0);
         }
         __syncwarp();
       }
     }
     if (!ok) pp.drain(q);
   } else if (warp == 1) {
-    // fp32 sums, both operands of one type, M = 128
+    // fp32 sums, both operands of one type, M = 256
     const uint32_t fmt = a.dtype == MOE_DT_BF16 ? 1u : 0u;
     const uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)kPMn << 15) |
                             ((uint32_t)kQMn << 16) | ((uint32_t)(kTM >> 4) << 24);
     int q = 0, j = 0;
-    for (int w = blockIdx.x; w < work.total; w += gridDim.x) {
+    for (int w = pair; w < work.total; w += pairs) {
       const Item it = work.item(w);
       const int nk = (it.len + kTK - 1) / kTK;
       if (nk == 0) continue;
       const int buf = j & 1;
-      if (j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
+      if (rank == 0 && j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
       fence_after_sync();
       const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
-      const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 15) >> 4) << 18);
+      const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 31) >> 5) << 19);
+      const int boxes = 2 + ((it.nc + 31) / 32 * 16 + 63) / 64;
       bool ok = true;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages;
@@ -164,17 +193,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         int steps = kTK / 16;
         if (kQMn && left < kTK) {
           steps = (left + 15) / 16;
-          const int nbox = 2 + (it.nc + 63) / 64, zr = steps * 16 - left;
-          for (int i = lane; i < nbox * zr * 8; i += 32) {
-            const int box = i / (zr * 8), r = left + i / 8 % zr;
-            *reinterpret_cast<uint4 *>(st + box * kMnBox + r * 128 + i % 8 * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          tma::fence_proxy_async_smem();
-          __syncwarp();
+          zero_rows(st, boxes, left, steps * 16);
         }
         fence_after_sync();
-        if (elect_one()) {
+        if (rank != 0) {
+          if (elect_one()) arrive_at(&pp.full[s], 0);
+        } else if (elect_one()) {
           const uint32_t base = su32(st);
           const uint64_t pd = kPMn ? sw128_desc(base, kMnBox, 1024) : sw128_desc(base, 16, 1024);
           const uint64_t qd = kQMn ? sw128_desc(base + kABytes, kMnBox, 1024)
@@ -184,30 +208,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (steps == kTK / 16) {
 #pragma unroll
             for (int k = 0; k < kTK / 16; ++k)
-              mma_f16(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+              mma_f16_pair(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
           } else {
             for (int k = 0; k < steps; ++k)
-              mma_f16(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+              mma_f16_pair(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
           }
-          commit(&pp.empty[s]);
+          commit_pair(&pp.empty[s]);
         }
         __syncwarp();
       }
       if (!ok) break;
-      if (elect_one()) commit(&pp.tfull[buf]);
+      if (rank == 0 && elect_one()) commit_pair(&pp.tfull[buf]);
       ++j;
     }
-    if (elect_one()) commit(&pp.done);
-  } else if (warp >= 2) {
+    // no MMA still runs, and no arrival is on its way, when the pair goes on
+    if (rank == 0 && elect_one()) commit_pair(&pp.done);
+    __syncwarp();
+    tma::mbar_wait(&pp.done, 0, nullptr);
+  } else {
     const int quarter = warp & 3, grp = (warp - 2) >> 2;
     uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kStages * kStageBytes +
                                                    (warp - 2) * kDrainBytes);
     const int M = KIND == kGroupedFwd ? a.n : a.k;
     const int64_t ld = KIND == kGroupedFwd ? a.ld_out : KIND == kGroupedDgrad ? a.ld_x : a.ld_w;
     int j = 0;
-    for (int w = blockIdx.x; w < work.total; w += gridDim.x) {
+    for (int w = pair; w < work.total; w += pairs) {
       const Item it = work.item(w);
-      const int m = it.m0 + quarter * 32;
+      const int m = it.m0 + rank * 128 + quarter * 32;
       const int64_t at = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
       const bool some = it.len > 0;
       const int buf = j & 1;
@@ -216,26 +243,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after_sync();
         ++j;
       }
-      const uint32_t trow =
-          pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16);
-      drain_tile(trow, some, it.nc, grp, M - m, a.out, a.out_dtype, at, ld, buf32);
+      if (m < M)
+        drain_tile(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), some,
+                   it.nc, grp, M - m, a.out, a.out_dtype, at, ld, buf32);
       if (some) {
         fence_before_sync();
         __syncwarp();
-        if (lane == 0) tma::mbar_arrive(&pp.tempty[buf]);
+        if (lane == 0) arrive_at(&pp.tempty[buf], 0);
       }
     }
   }
-  if (threadIdx.x == 32) tma::mbar_wait(&pp.done, 0, nullptr);  // no MMA still runs
+  __syncwarp();
   fence_before_sync();
-  __syncthreads();
+  cluster_sync();
   if (threadIdx.x == 0 && pp.abort_flag) set_status(a.status, kStatusTimeout);
-  if (warp == 1) tmem_dealloc(pp.tmem_base, 2 * kTN);
+  if (warp == 1) tmem_dealloc_pair(pp.tmem_base, 2 * kTN);
 }
 
 template <int KIND>
-cudaError_t launch_kind(const CUtensorMap &p, const CUtensorMap &q, const GroupedArgs &a,
-                        cudaStream_t s) {
+cudaError_t launch_kind(const CUtensorMap &p, const CUtensorMap &q, const CUtensorMap &q16,
+                        const GroupedArgs &a, cudaStream_t s) {
   static const cudaError_t attr = cudaFuncSetAttribute(
       grouped_tc_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   if (attr != cudaSuccess) return attr;
@@ -243,8 +270,8 @@ cudaError_t launch_kind(const CUtensorMap &p, const CUtensorMap &q, const Groupe
   const long long g = KIND == kGroupedWgrad ? (long long)a.E * ((a.n + kTN - 1) / kTN)
                                             : a.R / kTN + std::min(a.E, a.R);
   if (g * nM > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
-  const int grid = (int)std::min<long long>(g * nM, a.sm_count);
-  grouped_tc_kernel<KIND><<<grid, kThreads, kSmem, s>>>(p, q, a);
+  const int grid = 2 * (int)std::min<long long>(g * nM, a.sm_count / 2);
+  grouped_tc_kernel<KIND><<<grid, kThreads, kSmem, s>>>(p, q, q16, a);
   return cudaGetLastError();
 }
 
@@ -259,7 +286,7 @@ bool grouped_tc_ok(GroupedKind kind, const GroupedArgs &a) {
 }
 
 cudaError_t launch_grouped_tc(GroupedKind kind, const GroupedArgs &a, cudaStream_t s) {
-  CUtensorMap p, q;
+  CUtensorMap p, q, q16;
   const auto rows_map = [&](CUtensorMap *m, const void *t, int width, int64_t ld, int box) {
     return tc::encode_map3d(m, t, (uint64_t)width * 2, (uint64_t)a.R, 1, (uint64_t)ld * 2,
                             (uint64_t)ld * 2, (uint32_t)box);
@@ -267,17 +294,20 @@ cudaError_t launch_grouped_tc(GroupedKind kind, const GroupedArgs &a, cudaStream
   bool ok;
   if (kind == kGroupedWgrad) {
     ok = rows_map(&p, a.x, a.k, a.ld_x, kTK) && rows_map(&q, a.dout, a.n, a.ld_out, kTK);
+    q16 = q;  // not used
   } else {
+    const bool fwd = kind == kGroupedFwd;
+    const void *rows = fwd ? a.x : a.dout;
+    const int width = fwd ? a.k : a.n;
+    const int64_t ld = fwd ? a.ld_x : a.ld_out;
     ok = tc::encode_map3d(&p, a.w, (uint64_t)a.k * 2, (uint64_t)a.n, (uint64_t)a.E,
-                          (uint64_t)a.ld_w * 2, (uint64_t)a.es_w * 2,
-                          kind == kGroupedFwd ? kTM : kTK);
-    ok = ok && (kind == kGroupedFwd ? rows_map(&q, a.x, a.k, a.ld_x, kBoxRows)
-                                    : rows_map(&q, a.dout, a.n, a.ld_out, kBoxRows));
+                          (uint64_t)a.ld_w * 2, (uint64_t)a.es_w * 2, fwd ? kTM / 2 : kTK) &&
+         rows_map(&q, rows, width, ld, kBig) && rows_map(&q16, rows, width, ld, kSmall);
   }
   if (!ok) return cudaErrorInvalidValue;
-  if (kind == kGroupedFwd) return launch_kind<kGroupedFwd>(p, q, a, s);
-  if (kind == kGroupedDgrad) return launch_kind<kGroupedDgrad>(p, q, a, s);
-  return launch_kind<kGroupedWgrad>(p, q, a, s);
+  if (kind == kGroupedFwd) return launch_kind<kGroupedFwd>(p, q, q16, a, s);
+  if (kind == kGroupedDgrad) return launch_kind<kGroupedDgrad>(p, q, q16, a, s);
+  return launch_kind<kGroupedWgrad>(p, q, q16, a, s);
 }
 
 }  // namespace moe

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     it.m0 = (w - g * nM) * kTM;
     it.e = seg.expert_of(g, a.E);
     const int cnt = seg.rows(it.e), nt = seg.tile0[it.e + 1] - seg.tile0[it.e];
-    const int sz = tile_rows(cnt, nt), t = g - seg.tile0[it.e];
+    const int sz = tile_rows<16>(cnt, nt), t = g - seg.tile0[it.e];
     it.c0 = seg.off[it.e] + t * sz;
     it.nc = min(sz, cnt - t * sz);
     return it;

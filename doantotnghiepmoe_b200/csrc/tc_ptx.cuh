@@ -122,14 +122,14 @@ struct Pipe {
   uint32_t tmem_base;
   int abort_flag;
 
-  __device__ __forceinline__ void init(uint32_t full_count) {
+  __device__ __forceinline__ void init(uint32_t full_count, uint32_t tempty_count = kEpiWarps) {
     for (int s = 0; s < S; ++s) {
       tma::mbar_init(&full[s], full_count);
       tma::mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       tma::mbar_init(&tfull[b], 1);
-      tma::mbar_init(&tempty[b], kEpiWarps);
+      tma::mbar_init(&tempty[b], tempty_count);
     }
     tma::mbar_init(&done, 1);
     abort_flag = 0;
@@ -272,10 +272,66 @@ __device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int
 }
 
 // Rows of the t-th of nt row tiles of an expert with cnt rows: equal tiles, a
-// multiple of 16 (the MMA's step of N), so that 300 rows become 160 + 140
-// rather than 256 + 44.  No tile is empty: nt is ceil(cnt / (a multiple of 16)).
+// multiple of kStep (the MMA's step of N), so that 300 rows become 160 + 140
+// rather than 256 + 44.  No tile is empty: nt is ceil(cnt / kMax) with kMax at
+// least 8 kStep, so cnt / nt + kStep tiles of that many rows never cover cnt
+// with nt - 1 of them, and from 8 tiles on the size is kMax.
+template <int kStep>
 __device__ __forceinline__ int tile_rows(int cnt, int nt) {
-  return ((cnt + nt - 1) / nt + 15) & ~15;
+  return ((cnt + nt - 1) / nt + kStep - 1) & ~(kStep - 1);
+}
+
+// ---- pairs of CTAs (clusters of two, cta_group::2) ---------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// Arrives on the barrier at the same place in CTA `rank` of the cluster.  What it
+// tells of is copies and tensor memory, which their own mechanisms order; where
+// it tells of plain stores, they are fenced first (release and acquire at
+// cluster scope on every step made the pair kernel 2.5 times slower).
+__device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(su32(bar)),
+      "r"(rank)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   su32(dst_smem)),
+               "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+               : "memory");
+}
+// As commit, on the barrier at the same place in both CTAs of the pair.
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(su32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// M = 256 over the pair: each CTA's shared memory holds its 128 rows of A and
+// its half of the rows of B, at the same places, and its TMEM 128 rows of D.
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 }  // namespace tcp
