@@ -14,11 +14,11 @@
 // each CTA loads its 128 of M and half of the N side and keeps 128 rows of D.
 // Against a CTA's own 128 x 256 tile this moves 32 KB rather than 48 KB from L2
 // for the same products, and L2 to SM traffic is what bounded that kernel (54
-// bytes a cycle and SM).  One persistent CTA an SM: a warp keeps a ring of 6
+// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of 6
 // stages (64 elements of K of both sides) full by TMA across items, the even
-// CTA's second warp issues the pair's MMAs into two accumulator buffers of 256
+// CTA's issuing warp issues the pair's MMAs into two accumulator buffers of 256
 // TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
-// odd CTA's second warp passes on that its stage has landed.  Tiles that reach
+// odd CTA's issuing warp passes on that its stage has landed.  Tiles that reach
 // past a segment read other experts' rows and drop their columns; in wgrad,
 // where the rows are summed, the rows of the last K step that belong to others
 // are zeroed in shared memory before the MMA (zeros alone would not do on one
@@ -96,7 +96,6 @@ __device__ __forceinline__ void zero_rows(uint8_t *st, int boxes, int left, int 
       *reinterpret_cast<uint4 *>(st + i / 8 * kMnBox + r * 128 + i % 8 * 16) =
           make_uint4(0, 0, 0, 0);
   tma::fence_proxy_async_smem();
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");  // the other CTA's thread issues the MMA
   __syncwarp();
 }
 
@@ -114,17 +113,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  // full: the even CTA's also counts the odd one's stage; tempty: both CTAs drain
-  if (threadIdx.x == 0) pp.init(rank == 0 ? 2 : 1, 2 * kEpiWarps);
+  // full: both copying warps, and the odd CTA's stage in the even one; tempty:
+  // both CTAs drain
+  if (threadIdx.x == 0) pp.init(rank == 0 ? 3 : 2, 2 * kEpiWarps);
   if (warp == 1) tmem_alloc_pair(&pp.tmem_base, 2 * kTN);
-  if (warp == 2) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
+  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
   fence_before_sync();
   __syncthreads();
   cluster_sync();
   fence_after_sync();
   const Work<KIND> work(a, seg);
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     int q = 0;
     bool ok = true;
     for (int w = pair; w < work.total && ok; w += pairs) {
@@ -133,8 +133,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int half = (it.nc + 31) / 32 * 16, c0 = it.c0 + rank * half, m0 = it.m0 + rank * 128;
       const int nbig = kQMn ? (half + 63) / 64 : half / kBig;
       const int nsmall = kQMn ? 0 : half % kBig / kSmall;
-      const uint32_t bytes = kABytes + nbig * kMnBox + nsmall * kSmall * 128u;
       static_assert(kBig * 128 == kMnBox, "one box size");
+      const uint32_t bytes = warp == 0 ? kABytes : nbig * kMnBox + nsmall * kSmall * 128u;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
         ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
@@ -143,23 +143,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint8_t *st = tiles + s * kStageBytes;
           tma::mbar_expect_tx(&pp.full[s], bytes);
           const int kr = it.row0 + kb * kTK;  // first row of K of an MN-major tile
-          if (kPMn) {
-            for (int i = 0; i < 2; ++i)
-              tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (m0 + 64 * i) * 2, kr,
-                           kQMn ? 0 : it.e);
+          if (warp == 0) {
+            if (kPMn) {
+              for (int i = 0; i < 2; ++i)
+                tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (m0 + 64 * i) * 2, kr,
+                             kQMn ? 0 : it.e);
+            } else {
+              tma::load_3d(st, &mapP, &pp.full[s], kb * 128, m0, it.e);
+            }
           } else {
-            tma::load_3d(st, &mapP, &pp.full[s], kb * 128, m0, it.e);
+            st += kABytes;
+            for (int i = 0; i < nbig; ++i) {
+              if (kQMn)
+                tma::load_3d(st + i * kMnBox, &mapQ, &pp.full[s], (c0 + 64 * i) * 2, kr, 0);
+              else
+                tma::load_3d(st + i * kMnBox, &mapQ, &pp.full[s], kb * 128, c0 + i * kBig, 0);
+            }
+            for (int i = 0; i < nsmall; ++i)
+              tma::load_3d(st + nbig * kMnBox + i * kSmall * 128, &mapQ16, &pp.full[s], kb * 128,
+                           c0 + nbig * kBig + i * kSmall, 0);
           }
-          for (int i = 0; i < nbig; ++i) {
-            if (kQMn)
-              tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], (c0 + 64 * i) * 2, kr, 0);
-            else
-              tma::load_3d(st + kABytes + i * kMnBox, &mapQ, &pp.full[s], kb * 128,
-                           c0 + i * kBig, 0);
-          }
-          for (int i = 0; i < nsmall; ++i)
-            tma::load_3d(st + kABytes + nbig * kMnBox + i * kSmall * 128, &mapQ16, &pp.full[s],
-                         kb * 128, c0 + nbig * kBig + i * kSmall, 0);
         }
         __syncwarp();
       }
@@ -193,11 +196,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         int steps = kTK / 16;
         if (kQMn && left < kTK) {
           steps = (left + 15) / 16;
-          zero_rows(st, boxes, left, steps * 16);
+          if (left % 16) zero_rows(st, boxes, left, steps * 16);
         }
         fence_after_sync();
         if (rank != 0) {
-          if (elect_one()) arrive_at(&pp.full[s], 0);
+          if (elect_one()) {
+            if (kQMn && left % 16) arrive_release_at(&pp.full[s], 0);
+            else arrive_at(&pp.full[s], 0);
+          }
         } else if (elect_one()) {
           const uint32_t base = su32(st);
           const uint64_t pd = kPMn ? sw128_desc(base, kMnBox, 1024) : sw128_desc(base, 16, 1024);
@@ -226,9 +232,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __syncwarp();
     tma::mbar_wait(&pp.done, 0, nullptr);
   } else {
-    const int quarter = warp & 3, grp = (warp - 2) >> 2;
+    const int quarter = warp & 3, grp = (warp - 3) >> 2;
     uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kStages * kStageBytes +
-                                                   (warp - 2) * kDrainBytes);
+                                                   (warp - 3) * kDrainBytes);
     const int M = KIND == kGroupedFwd ? a.n : a.k;
     const int64_t ld = KIND == kGroupedFwd ? a.ld_out : KIND == kGroupedDgrad ? a.ld_x : a.ld_w;
     int j = 0;

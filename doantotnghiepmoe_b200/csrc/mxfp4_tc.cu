@@ -33,7 +33,7 @@ using namespace tcp;
 constexpr int kTM = 128, kTN = 192;
 constexpr int kStages = 4;
 constexpr uint32_t kABytes = kTM * 128, kBBytes = kTN * 128, kStageBytes = kABytes + kBBytes;
-constexpr int kBoxRows = 32;
+constexpr int kBig = 64, kSmall = 16;  // rows of x of one copy
 constexpr int kGroup = 512;            // scale bytes of 128 rows and 4 blocks
 constexpr int kScaleBytes = 6 * kGroup;  // of a stage: 2 groups of w, 2 x 2 of x
 constexpr int kSetCols = 24;             // TMEM columns of a stage's scales
@@ -47,7 +47,8 @@ static_assert(kSmem <= 232448, "shared memory");
 
 __global__ void __launch_bounds__(kMxThreads, 1)
     mxfp4_tc_kernel(const __grid_constant__ CUtensorMap mapW,
-                    const __grid_constant__ CUtensorMap mapX, Mxfp4Args a) {
+                    const __grid_constant__ CUtensorMap mapX,
+                    const __grid_constant__ CUtensorMap mapX16, Mxfp4Args a) {
   extern __shared__ uint8_t smem_raw[];
   using P = Pipe<kStages>;
   P &pp = *reinterpret_cast<P *>(smem_raw);
@@ -55,9 +56,9 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
   uint8_t *scales = tiles + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) pp.init(1 + 32);  // the copying thread, a scale warp's lanes
+  if (threadIdx.x == 0) pp.init(2 + 32);  // the copying warps, a scale warp's lanes
   if (warp == 1) tmem_alloc(&pp.tmem_base, kTmemCols);
-  if (warp == 2) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
+  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -79,23 +80,30 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     return it;
   };
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     int q = 0;
     bool ok = true;
     for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
       const Item it = item(w);
-      const int nbox = (it.nc + kBoxRows - 1) / kBoxRows;
+      const int nbig = it.nc / kBig, nsmall = (it.nc % kBig + kSmall - 1) / kSmall;
+      const uint32_t bytes = warp == 0 ? kABytes : (nbig * kBig + nsmall * kSmall) * 128u;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
         ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
           uint8_t *st = tiles + s * kStageBytes;
-          tma::mbar_expect_tx(&pp.full[s], kABytes + nbox * kBoxRows * 128u);
-          tma::load_3d(st, &mapW, &pp.full[s], kb * 128, it.m0, it.e);
-          for (int i = 0; i < nbox; ++i)
-            tma::load_3d(st + kABytes + i * kBoxRows * 128, &mapX, &pp.full[s], kb * 128,
-                         it.c0 + i * kBoxRows, 0);
+          tma::mbar_expect_tx(&pp.full[s], bytes);
+          if (warp == 0) {
+            tma::load_3d(st, &mapW, &pp.full[s], kb * 128, it.m0, it.e);
+          } else {
+            st += kABytes;
+            for (int i = 0; i < nbig; ++i)
+              tma::load_3d(st + i * kBig * 128, &mapX, &pp.full[s], kb * 128, it.c0 + i * kBig, 0);
+            for (int i = 0; i < nsmall; ++i)
+              tma::load_3d(st + (nbig * kBig + i * kSmall) * 128, &mapX16, &pp.full[s], kb * 128,
+                           it.c0 + nbig * kBig + i * kSmall, 0);
+          }
         }
         __syncwarp();
       }
@@ -146,13 +154,13 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       if (elect_one()) commit(&pp.tfull[buf]);
     }
     if (elect_one()) commit(&pp.done);
-  } else if (warp >= 2 && warp < 2 + kScaleWarps) {
+  } else if (warp < 3 + kScaleWarps) {
     const int words = mxfp4_scale_stride(a.k) / 4;
     const uint32_t *xs = reinterpret_cast<const uint32_t *>(a.xs);
     const uint32_t *ws = reinterpret_cast<const uint32_t *>(a.ws);
     int w = blockIdx.x;
-    int kb = warp - 2;  // this warp's steps: every kScaleWarps-th
-    for (int q = warp - 2;; q += kScaleWarps, kb += kScaleWarps) {
+    int kb = warp - 3;  // this warp's steps: every kScaleWarps-th
+    for (int q = warp - 3;; q += kScaleWarps, kb += kScaleWarps) {
       for (; kb >= nk && w < total; kb -= nk) w += gridDim.x;
       if (w >= total) break;
       const Item it = item(w);
@@ -180,8 +188,8 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       tma::fence_proxy_async_smem();  // before the tensor cores' proxy reads them
       tma::mbar_arrive(&pp.full[s]);
     }
-  } else if (warp >= 2) {
-    const int ew = warp - 2 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
+  } else {
+    const int ew = warp - 3 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
     uint32_t *buf32 = reinterpret_cast<uint32_t *>(scales + kStages * kScaleBytes +
                                                    ew * kDrainBytes);
     int j = 0;
@@ -212,13 +220,14 @@ cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
       mxfp4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   if (attr != cudaSuccess) return attr;
   const uint64_t row = (uint64_t)mxfp4_code_stride(a.k);
-  CUtensorMap w, x;
+  CUtensorMap w, x, x16;
   if (!tc::encode_map3d(&w, a.wc, row, (uint64_t)a.n, (uint64_t)a.E, row, row * a.n, kTM) ||
-      !tc::encode_map3d(&x, a.xc, row, (uint64_t)a.R, 1, row, row, kBoxRows))
+      !tc::encode_map3d(&x, a.xc, row, (uint64_t)a.R, 1, row, row, kBig) ||
+      !tc::encode_map3d(&x16, a.xc, row, (uint64_t)a.R, 1, row, row, kSmall))
     return cudaErrorInvalidValue;
   const long long items = (long long)(a.R / kTN + std::min(a.E, a.R)) * ((a.n + kTM - 1) / kTM);
   if (items > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
-  mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(w, x, a);
+  mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(w, x, x16, a);
   return cudaGetLastError();
 }
 

@@ -1,6 +1,6 @@
 // PTX wrappers of the tensor-core instructions (tcgen05) that the grouped
 // products use, their descriptors, and the barriers of a persistent kernel
-// with one copying thread, one issuing warp and kEpiWarps draining warps.
+// with two copying warps, one issuing warp and kEpiWarps draining warps.
 #pragma once
 
 #include <cstdint>
@@ -111,8 +111,11 @@ __device__ __forceinline__ uint64_t rows16_desc(uint32_t saddr) {
 }
 
 
-constexpr int kEpiWarps = 16;                  // four a TMEM lane quarter
-constexpr int kThreads = 64 + 32 * kEpiWarps;  // and the copying and issuing warps
+// Warps: 0 copies the M side, 1 issues the MMAs, 2 copies the N side (a copy
+// takes 60 to 70 cycles to issue, and one warp for both was the bound), and
+// then, behind any others of a kernel, the draining warps.
+constexpr int kEpiWarps = 16;  // four a TMEM lane quarter
+constexpr int kThreads = 96 + 32 * kEpiWarps;
 
 template <int S>
 struct Pipe {
@@ -200,10 +203,12 @@ __device__ __forceinline__ void store_cols(T *out, int64_t ld, int nc, int left,
     __syncwarp();
     return;
   }
+  const bool whole = nc >= 32 && left >= 32;  // nothing to leave out
   if constexpr (sizeof(T) == 2) {
     const int p = lane / 4, m = lane % 4 * 8;
+    T *row = out + 2 * p * ld + m;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h, row += 16 * ld) {
       if (16 * h >= nc) break;  // warp-uniform
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -212,33 +217,39 @@ __device__ __forceinline__ void store_cols(T *out, int64_t ld, int nc, int left,
       __syncwarp();
       const uint4 a = *reinterpret_cast<const uint4 *>(buf + p * 32 + m);
       const uint4 b = *reinterpret_cast<const uint4 *>(buf + p * 32 + m + 4);
-      const int i = 16 * h + 2 * p;
-      T *row = out + i * ld + m;
-      if (i < nc)
-        store_piece(row, make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
-                                    __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410)),
-                    left - m);
-      if (i + 1 < nc)
-        store_piece(row + ld,
-                    make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
-                               __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632)),
-                    left - m);
+      const uint4 lo =
+          make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                     __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+      const uint4 hi =
+          make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                     __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
+      if (whole) {
+        *reinterpret_cast<uint4 *>(row) = lo;
+        *reinterpret_cast<uint4 *>(row + ld) = hi;
+      } else {
+        const int i = 16 * h + 2 * p;
+        if (i < nc) store_piece(row, lo, left - m);
+        if (i + 1 < nc) store_piece(row + ld, hi, left - m);
+      }
       __syncwarp();
     }
   } else {
-    const int m = lane % 8 * 4;
+    const int r = lane / 8, m = lane % 8 * 4;
+    T *row = out + r * ld + m;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
+    for (int h = 0; h < 4; ++h, row += 8 * ld) {
       if (8 * h >= nc) break;  // warp-uniform
 #pragma unroll
       for (int i = 0; i < 8; ++i) buf[i * 32 + lane] = v[8 * h + i];
       __syncwarp();
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int r = lane / 8 + 4 * t, i = 8 * h + r;
-        if (i < nc)
-          store_piece(out + i * ld + m, *reinterpret_cast<const uint4 *>(buf + r * 32 + m),
-                      left - m);
+      const uint4 lo = *reinterpret_cast<const uint4 *>(buf + r * 32 + m);
+      const uint4 hi = *reinterpret_cast<const uint4 *>(buf + (r + 4) * 32 + m);
+      if (whole) {
+        *reinterpret_cast<uint4 *>(row) = lo;
+        *reinterpret_cast<uint4 *>(row + 4 * ld) = hi;
+      } else {
+        if (8 * h + r < nc) store_piece(row, lo, left - m);
+        if (8 * h + r + 4 < nc) store_piece(row + 4 * ld, hi, left - m);
       }
       __syncwarp();
     }
@@ -293,13 +304,21 @@ __device__ __forceinline__ void cluster_sync() {
 }
 // Arrives on the barrier at the same place in CTA `rank` of the cluster.  What it
 // tells of is copies and tensor memory, which their own mechanisms order; where
-// it tells of plain stores, they are fenced first (release and acquire at
+// it tells of plain stores, arrive_release_at is used (release and acquire at
 // cluster scope on every step made the pair kernel 2.5 times slower).
 __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
   asm volatile(
       "{\n\t.reg .b32 a;\n\t"
       "mapa.shared::cluster.u32 a, %0, %1;\n\t"
       "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(su32(bar)),
+      "r"(rank)
+      : "memory");
+}
+__device__ __forceinline__ void arrive_release_at(uint64_t *bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(su32(bar)),
       "r"(rank)
       : "memory");
 }
