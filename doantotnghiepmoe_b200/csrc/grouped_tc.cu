@@ -20,9 +20,11 @@
 // TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
 // odd CTA's issuing warp passes on that its stage has landed.  Tiles that reach
 // past a segment read other experts' rows and drop their columns; in wgrad,
-// where the rows are summed, the rows of the last K step that belong to others
-// are zeroed in shared memory before the MMA (zeros alone would not do on one
-// side: 0 x NaN).  Every wait on a barrier in memory is bounded, as in
+// where the rows are summed, the last K step's rows beyond the expert's must be
+// zeros on both sides (0 x NaN): that step's copies are cut to 16, 4 and 1 rows,
+// and the rows up to the MMA's 16 come from behind the tensor's last row, where a
+// copy reads zeros.  (Zeroing them in shared memory cost the step two fences, 2000
+// cycles in the even CTA and 11000 in the odd one while results were stored.)  Every wait on a barrier in memory is bounded, as in
 // expert_tc.cu.
 #include <cuda.h>
 
@@ -41,8 +43,14 @@ using namespace tcp;
 constexpr int kTM = 256, kTN = 256, kTK = 64;  // tile of a pair; kTK elements are 128 bytes
 constexpr int kStages = 6;
 constexpr uint32_t kABytes = kTM / 2 * 128, kStageBytes = (kTM + kTN) / 2 * 128;  // of a CTA
-constexpr int kBig = 64, kSmall = 16;     // N-side rows of one copy (K-major)
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
+
+// Tensor maps: the M side and the N side with rows in boxes of several heights.
+//   forward, dgrad  p[0] all of a tile; q[0..2] 64, 32 and 16 rows
+//   wgrad           p[0..3], q[0..3]: 64, 16, 4 and 1 rows
+struct Maps {
+  CUtensorMap p[4], q[4];
+};
 constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
                          (size_t)kStages * kStageBytes + kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
@@ -88,22 +96,34 @@ struct Work {
   }
 };
 
-// Zeroes K rows [left, to) of the `boxes` MN-major copies of a stage.
-__device__ __forceinline__ void zero_rows(uint8_t *st, int boxes, int left, int to) {
-  const int lane = threadIdx.x & 31;
-  for (int r = left; r < to; ++r)
-    for (int i = lane; i < boxes * 8; i += 32)
-      *reinterpret_cast<uint4 *>(st + i / 8 * kMnBox + r * 128 + i % 8 * 16) =
-          make_uint4(0, 0, 0, 0);
-  tma::fence_proxy_async_smem();
-  __syncwarp();
+// The copies of an MN-major side's K step: rows [row, row + 64) of `boxes`
+// columns of 64 elements from col on, or, where only left < 64 of them belong
+// to the sum, those and zeros up to a multiple of 16.  zero: a row behind the
+// tensor.
+__device__ __forceinline__ void load_mn(uint8_t *st, const CUtensorMap (&m)[4], uint64_t *bar,
+                                        int col, int boxes, int row, int left, int zero) {
+  if (left >= kTK) {
+    for (int i = 0; i < boxes; ++i)
+      tma::load_3d(st + i * kMnBox, &m[0], bar, (col + 64 * i) * 2, row, 0);
+    return;
+  }
+  for (int i = 0; i < boxes; ++i) {
+    const int x = (col + 64 * i) * 2;
+    uint8_t *dst = st + i * kMnBox;
+    int r = 0;
+    for (; r + 16 <= left; r += 16) tma::load_3d(dst + r * 128, &m[1], bar, x, row + r, 0);
+    if (r == left) continue;
+    const int end = r + 16;
+    for (; r + 4 <= left; r += 4) tma::load_3d(dst + r * 128, &m[2], bar, x, row + r, 0);
+    for (; r & 3 || r < left; ++r)
+      tma::load_3d(dst + r * 128, &m[3], bar, x, r < left ? row + r : zero, 0);
+    for (; r < end; r += 4) tma::load_3d(dst + r * 128, &m[2], bar, x, zero, 0);
+  }
 }
 
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    grouped_tc_kernel(const __grid_constant__ CUtensorMap mapP,
-                      const __grid_constant__ CUtensorMap mapQ,
-                      const __grid_constant__ CUtensorMap mapQ16, GroupedArgs a) {
+    grouped_tc_kernel(const __grid_constant__ Maps maps, const GroupedArgs a) {
   constexpr bool kPMn = KIND != kGroupedFwd, kQMn = KIND == kGroupedWgrad;
   extern __shared__ uint8_t smem_raw[];
   using P = Pipe<kStages>;
@@ -113,9 +133,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  // full: both copying warps, and the odd CTA's stage in the even one; tempty:
-  // both CTAs drain
-  if (threadIdx.x == 0) pp.init(rank == 0 ? 3 : 2, 2 * kEpiWarps);
+  // full: the M side's copying warp (for both), and the odd CTA's stage in the
+  // even one; tempty: both CTAs drain
+  if (threadIdx.x == 0) pp.init(rank == 0 ? 2 : 1, 2 * kEpiWarps);
   if (warp == 1) tmem_alloc_pair(&pp.tmem_base, 2 * kTN);
   if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
   fence_before_sync();
@@ -131,37 +151,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item it = work.item(w);
       const int nk = (it.len + kTK - 1) / kTK;
       const int half = (it.nc + 31) / 32 * 16, c0 = it.c0 + rank * half, m0 = it.m0 + rank * 128;
-      const int nbig = kQMn ? (half + 63) / 64 : half / kBig;
-      const int nsmall = kQMn ? 0 : half % kBig / kSmall;
-      static_assert(kBig * 128 == kMnBox, "one box size");
-      const uint32_t bytes = warp == 0 ? kABytes : nbig * kMnBox + nsmall * kSmall * 128u;
+      const int boxes = (half + 63) / 64;  // of an MN-major N side
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
         ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
           uint8_t *st = tiles + s * kStageBytes;
-          tma::mbar_expect_tx(&pp.full[s], bytes);
+          uint64_t *bar = &pp.full[s];
           const int kr = it.row0 + kb * kTK;  // first row of K of an MN-major tile
+          const int left = kQMn ? it.len - kb * kTK : kTK;
           if (warp == 0) {
-            if (kPMn) {
-              for (int i = 0; i < 2; ++i)
-                tma::load_3d(st + i * kMnBox, &mapP, &pp.full[s], (m0 + 64 * i) * 2, kr,
-                             kQMn ? 0 : it.e);
+            tma::mbar_expect_tx(bar, kQMn ? (2 + boxes) * 128u * min(kTK, (left + 15) & ~15)
+                                          : kABytes + half * 128u);
+            if (KIND == kGroupedFwd) {
+              tma::load_3d(st, &maps.p[0], bar, kb * 128, m0, it.e);
+            } else if (KIND == kGroupedDgrad) {
+              tma::load_3d(st, &maps.p[0], bar, m0 * 2, kr, it.e);
+              tma::load_3d(st + kMnBox, &maps.p[0], bar, m0 * 2 + 128, kr, it.e);
             } else {
-              tma::load_3d(st, &mapP, &pp.full[s], kb * 128, m0, it.e);
+              load_mn(st, maps.p, bar, m0, 2, kr, left, a.R);
             }
           } else {
             st += kABytes;
-            for (int i = 0; i < nbig; ++i) {
-              if (kQMn)
-                tma::load_3d(st + i * kMnBox, &mapQ, &pp.full[s], (c0 + 64 * i) * 2, kr, 0);
-              else
-                tma::load_3d(st + i * kMnBox, &mapQ, &pp.full[s], kb * 128, c0 + i * kBig, 0);
+            if (kQMn) {
+              load_mn(st, maps.q, bar, c0, boxes, kr, left, a.R);
+            } else {
+              if (half & 192) tma::load_3d(st, &maps.q[0], bar, kb * 128, c0, 0);
+              if (half & 128) tma::load_3d(st + 64 * 128, &maps.q[0], bar, kb * 128, c0 + 64, 0);
+              if (half & 32)
+                tma::load_3d(st + (half & 64) * 128, &maps.q[1], bar, kb * 128, c0 + (half & 64), 0);
+              if (half & 16)
+                tma::load_3d(st + (half & 96) * 128, &maps.q[2], bar, kb * 128, c0 + (half & 96), 0);
             }
-            for (int i = 0; i < nsmall; ++i)
-              tma::load_3d(st + nbig * kMnBox + i * kSmall * 128, &mapQ16, &pp.full[s], kb * 128,
-                           c0 + nbig * kBig + i * kSmall, 0);
           }
         }
         __syncwarp();
@@ -183,7 +205,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       fence_after_sync();
       const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 31) >> 5) << 19);
-      const int boxes = 2 + ((it.nc + 31) / 32 * 16 + 63) / 64;
       bool ok = true;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages;
@@ -192,18 +213,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           break;
         }
         uint8_t *st = tiles + s * kStageBytes;
-        const int left = it.len - kb * kTK;  // elements of K that belong to the sum
-        int steps = kTK / 16;
-        if (kQMn && left < kTK) {
-          steps = (left + 15) / 16;
-          if (left % 16) zero_rows(st, boxes, left, steps * 16);
-        }
+        const int steps = kQMn ? min(kTK, it.len - kb * kTK + 15) / 16 : kTK / 16;
         fence_after_sync();
         if (rank != 0) {
-          if (elect_one()) {
-            if (kQMn && left % 16) arrive_release_at(&pp.full[s], 0);
-            else arrive_at(&pp.full[s], 0);
-          }
+          if (elect_one()) arrive_at(&pp.full[s], 0);
         } else if (elect_one()) {
           const uint32_t base = su32(st);
           const uint64_t pd = kPMn ? sw128_desc(base, kMnBox, 1024) : sw128_desc(base, 16, 1024);
@@ -267,8 +280,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 template <int KIND>
-cudaError_t launch_kind(const CUtensorMap &p, const CUtensorMap &q, const CUtensorMap &q16,
-                        const GroupedArgs &a, cudaStream_t s) {
+cudaError_t launch_kind(const Maps &maps, const GroupedArgs &a, cudaStream_t s) {
   static const cudaError_t attr = cudaFuncSetAttribute(
       grouped_tc_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   if (attr != cudaSuccess) return attr;
@@ -277,7 +289,7 @@ cudaError_t launch_kind(const CUtensorMap &p, const CUtensorMap &q, const CUtens
                                             : a.R / kTN + std::min(a.E, a.R);
   if (g * nM > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
   const int grid = 2 * (int)std::min<long long>(g * nM, a.sm_count / 2);
-  grouped_tc_kernel<KIND><<<grid, kThreads, kSmem, s>>>(p, q, q16, a);
+  grouped_tc_kernel<KIND><<<grid, kThreads, kSmem, s>>>(maps, a);
   return cudaGetLastError();
 }
 
@@ -292,28 +304,29 @@ bool grouped_tc_ok(GroupedKind kind, const GroupedArgs &a) {
 }
 
 cudaError_t launch_grouped_tc(GroupedKind kind, const GroupedArgs &a, cudaStream_t s) {
-  CUtensorMap p, q, q16;
+  Maps maps;
   const auto rows_map = [&](CUtensorMap *m, const void *t, int width, int64_t ld, int box) {
     return tc::encode_map3d(m, t, (uint64_t)width * 2, (uint64_t)a.R, 1, (uint64_t)ld * 2,
                             (uint64_t)ld * 2, (uint32_t)box);
   };
-  bool ok;
+  bool ok = true;
   if (kind == kGroupedWgrad) {
-    ok = rows_map(&p, a.x, a.k, a.ld_x, kTK) && rows_map(&q, a.dout, a.n, a.ld_out, kTK);
-    q16 = q;  // not used
+    const int heights[4] = {kTK, 16, 4, 1};
+    for (int i = 0; i < 4; ++i)
+      ok = ok && rows_map(&maps.p[i], a.x, a.k, a.ld_x, heights[i]) &&
+           rows_map(&maps.q[i], a.dout, a.n, a.ld_out, heights[i]);
   } else {
     const bool fwd = kind == kGroupedFwd;
-    const void *rows = fwd ? a.x : a.dout;
-    const int width = fwd ? a.k : a.n;
-    const int64_t ld = fwd ? a.ld_x : a.ld_out;
-    ok = tc::encode_map3d(&p, a.w, (uint64_t)a.k * 2, (uint64_t)a.n, (uint64_t)a.E,
-                          (uint64_t)a.ld_w * 2, (uint64_t)a.es_w * 2, fwd ? kTM / 2 : kTK) &&
-         rows_map(&q, rows, width, ld, kBig) && rows_map(&q16, rows, width, ld, kSmall);
+    ok = tc::encode_map3d(&maps.p[0], a.w, (uint64_t)a.k * 2, (uint64_t)a.n, (uint64_t)a.E,
+                          (uint64_t)a.ld_w * 2, (uint64_t)a.es_w * 2, fwd ? kTM / 2 : kTK);
+    for (int i = 0; i < 3; ++i)
+      ok = ok && rows_map(&maps.q[i], fwd ? a.x : a.dout, fwd ? a.k : a.n,
+                          fwd ? a.ld_x : a.ld_out, 64 >> i);
   }
   if (!ok) return cudaErrorInvalidValue;
-  if (kind == kGroupedFwd) return launch_kind<kGroupedFwd>(p, q, q16, a, s);
-  if (kind == kGroupedDgrad) return launch_kind<kGroupedDgrad>(p, q, q16, a, s);
-  return launch_kind<kGroupedWgrad>(p, q, q16, a, s);
+  if (kind == kGroupedFwd) return launch_kind<kGroupedFwd>(maps, a, s);
+  if (kind == kGroupedDgrad) return launch_kind<kGroupedDgrad>(maps, a, s);
+  return launch_kind<kGroupedWgrad>(maps, a, s);
 }
 
 }  // namespace moe

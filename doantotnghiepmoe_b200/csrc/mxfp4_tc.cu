@@ -33,7 +33,6 @@ using namespace tcp;
 constexpr int kTM = 128, kTN = 192;
 constexpr int kStages = 4;
 constexpr uint32_t kABytes = kTM * 128, kBBytes = kTN * 128, kStageBytes = kABytes + kBBytes;
-constexpr int kBig = 64, kSmall = 16;  // rows of x of one copy
 constexpr int kGroup = 512;            // scale bytes of 128 rows and 4 blocks
 constexpr int kScaleBytes = 6 * kGroup;  // of a stage: 2 groups of w, 2 x 2 of x
 constexpr int kSetCols = 24;             // TMEM columns of a stage's scales
@@ -45,10 +44,12 @@ constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
                          (size_t)kStages * (kStageBytes + kScaleBytes) + kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
 
+struct Maps {
+  CUtensorMap w, x[3];  // x in boxes of 64, 32 and 16 rows
+};
+
 __global__ void __launch_bounds__(kMxThreads, 1)
-    mxfp4_tc_kernel(const __grid_constant__ CUtensorMap mapW,
-                    const __grid_constant__ CUtensorMap mapX,
-                    const __grid_constant__ CUtensorMap mapX16, Mxfp4Args a) {
+    mxfp4_tc_kernel(const __grid_constant__ Maps maps, const Mxfp4Args a) {
   extern __shared__ uint8_t smem_raw[];
   using P = Pipe<kStages>;
   P &pp = *reinterpret_cast<P *>(smem_raw);
@@ -56,7 +57,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
   uint8_t *scales = tiles + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) pp.init(2 + 32);  // the copying warps, a scale warp's lanes
+  if (threadIdx.x == 0) pp.init(1 + 32);  // a copying warp (for both), a scale warp's lanes
   if (warp == 1) tmem_alloc(&pp.tmem_base, kTmemCols);
   if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
   fence_before_sync();
@@ -85,24 +86,27 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     bool ok = true;
     for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
       const Item it = item(w);
-      const int nbig = it.nc / kBig, nsmall = (it.nc % kBig + kSmall - 1) / kSmall;
-      const uint32_t bytes = warp == 0 ? kABytes : (nbig * kBig + nsmall * kSmall) * 128u;
+      const int rows = (it.nc + 15) & ~15;
       for (int kb = 0; kb < nk; ++kb, ++q) {
         const int s = q % kStages, use = q / kStages;
         ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
           uint8_t *st = tiles + s * kStageBytes;
-          tma::mbar_expect_tx(&pp.full[s], bytes);
+          uint64_t *bar = &pp.full[s];
           if (warp == 0) {
-            tma::load_3d(st, &mapW, &pp.full[s], kb * 128, it.m0, it.e);
+            tma::mbar_expect_tx(bar, kABytes + rows * 128u);
+            tma::load_3d(st, &maps.w, bar, kb * 128, it.m0, it.e);
           } else {
             st += kABytes;
-            for (int i = 0; i < nbig; ++i)
-              tma::load_3d(st + i * kBig * 128, &mapX, &pp.full[s], kb * 128, it.c0 + i * kBig, 0);
-            for (int i = 0; i < nsmall; ++i)
-              tma::load_3d(st + (nbig * kBig + i * kSmall) * 128, &mapX16, &pp.full[s], kb * 128,
-                           it.c0 + nbig * kBig + i * kSmall, 0);
+            for (int r = 0; r + 64 <= rows; r += 64)
+              tma::load_3d(st + r * 128, &maps.x[0], bar, kb * 128, it.c0 + r, 0);
+            if (rows & 32)
+              tma::load_3d(st + (rows & 192) * 128, &maps.x[1], bar, kb * 128,
+                           it.c0 + (rows & 192), 0);
+            if (rows & 16)
+              tma::load_3d(st + (rows & 224) * 128, &maps.x[2], bar, kb * 128,
+                           it.c0 + (rows & 224), 0);
           }
         }
         __syncwarp();
@@ -220,14 +224,14 @@ cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
       mxfp4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   if (attr != cudaSuccess) return attr;
   const uint64_t row = (uint64_t)mxfp4_code_stride(a.k);
-  CUtensorMap w, x, x16;
-  if (!tc::encode_map3d(&w, a.wc, row, (uint64_t)a.n, (uint64_t)a.E, row, row * a.n, kTM) ||
-      !tc::encode_map3d(&x, a.xc, row, (uint64_t)a.R, 1, row, row, kBig) ||
-      !tc::encode_map3d(&x16, a.xc, row, (uint64_t)a.R, 1, row, row, kSmall))
-    return cudaErrorInvalidValue;
+  Maps maps;
+  bool ok = tc::encode_map3d(&maps.w, a.wc, row, (uint64_t)a.n, (uint64_t)a.E, row, row * a.n, kTM);
+  for (int i = 0; i < 3; ++i)
+    ok = ok && tc::encode_map3d(&maps.x[i], a.xc, row, (uint64_t)a.R, 1, row, row, 64 >> i);
+  if (!ok) return cudaErrorInvalidValue;
   const long long items = (long long)(a.R / kTN + std::min(a.E, a.R)) * ((a.n + kTM - 1) / kTM);
   if (items > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
-  mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(w, x, x16, a);
+  mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(maps, a);
   return cudaGetLastError();
 }
 

@@ -303,22 +303,14 @@ __device__ __forceinline__ void cluster_sync() {
                    : "memory");
 }
 // Arrives on the barrier at the same place in CTA `rank` of the cluster.  What it
-// tells of is copies and tensor memory, which their own mechanisms order; where
-// it tells of plain stores, arrive_release_at is used (release and acquire at
-// cluster scope on every step made the pair kernel 2.5 times slower).
+// tells of is copies and tensor memory, which their own mechanisms order, never
+// plain stores (release and acquire at cluster scope on every step made the pair
+// kernel 2.5 times slower).
 __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
   asm volatile(
       "{\n\t.reg .b32 a;\n\t"
       "mapa.shared::cluster.u32 a, %0, %1;\n\t"
       "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(su32(bar)),
-      "r"(rank)
-      : "memory");
-}
-__device__ __forceinline__ void arrive_release_at(uint64_t *bar, uint32_t rank) {
-  asm volatile(
-      "{\n\t.reg .b32 a;\n\t"
-      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
-      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(su32(bar)),
       "r"(rank)
       : "memory");
 }
