@@ -14,8 +14,10 @@
 // each CTA loads its 128 of M and half of the N side and keeps 128 rows of D.
 // Against a CTA's own 128 x 256 tile this moves 32 KB rather than 48 KB from L2
 // for the same products, and L2 to SM traffic is what bounded that kernel (54
-// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of 6
-// stages (64 elements of K of both sides) full by TMA across items, the even
+// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of 3
+// stages (128 elements of K of both sides; 6 of 64 cost a wait, a commit and an
+// election twice as often, 560 cycles a 64 where the MMAs take 2 N) full by TMA
+// across items, the even
 // CTA's issuing warp issues the pair's MMAs into two accumulator buffers of 256
 // TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
 // odd CTA's issuing warp passes on that its stage has landed.  Tiles that reach
@@ -41,8 +43,9 @@ namespace {
 using namespace tcp;
 
 constexpr int kTM = 256, kTN = 256, kTK = 64;  // tile of a pair; kTK elements are 128 bytes
-constexpr int kStages = 6;
-constexpr uint32_t kABytes = kTM / 2 * 128, kStageBytes = (kTM + kTN) / 2 * 128;  // of a CTA
+constexpr int kStages = 6, kSub = 1;  // a stage holds kSub times kTK
+constexpr uint32_t kABytes = kTM / 2 * 128, kSubBytes = (kTM + kTN) / 2 * 128;  // of a CTA
+constexpr uint32_t kStageBytes = kSub * kSubBytes;
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.
@@ -145,94 +148,102 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const Work<KIND> work(a, seg);
 
   if (warp == 0 || warp == 2) {
-    int q = 0;
+    Ring<kStages> ring;
     bool ok = true;
     for (int w = pair; w < work.total && ok; w += pairs) {
       const Item it = work.item(w);
-      const int nk = (it.len + kTK - 1) / kTK;
       const int half = (it.nc + 31) / 32 * 16, c0 = it.c0 + rank * half, m0 = it.m0 + rank * 128;
       const int boxes = (half + 63) / 64;  // of an MN-major N side
-      for (int kb = 0; kb < nk; ++kb, ++q) {
-        const int s = q % kStages, use = q / kStages;
-        ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
+      for (int k0 = 0; k0 < it.len; k0 += kSub * kTK, ring.next()) {
+        ok = ring.use == 0 || pp.wait_warp(&pp.empty[ring.s], (ring.use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t *st = tiles + s * kStageBytes;
-          uint64_t *bar = &pp.full[s];
-          const int kr = it.row0 + kb * kTK;  // first row of K of an MN-major tile
-          const int left = kQMn ? it.len - kb * kTK : kTK;
-          if (warp == 0) {
-            tma::mbar_expect_tx(bar, kQMn ? (2 + boxes) * 128u * min(kTK, (left + 15) & ~15)
-                                          : kABytes + half * 128u);
-            if (KIND == kGroupedFwd) {
-              tma::load_3d(st, &maps.p[0], bar, kb * 128, m0, it.e);
-            } else if (KIND == kGroupedDgrad) {
-              tma::load_3d(st, &maps.p[0], bar, m0 * 2, kr, it.e);
-              tma::load_3d(st + kMnBox, &maps.p[0], bar, m0 * 2 + 128, kr, it.e);
+          uint8_t *st = tiles + ring.s * kStageBytes;
+          uint64_t *bar = &pp.full[ring.s];
+          const int left = it.len - k0;  // of the summed axis
+          if (warp == 0)
+            tma::mbar_expect_tx(
+                bar, kQMn ? (2 + boxes) * 128u * min(kSub * kTK, (left + 15) & ~15)
+                          : (kABytes + half * 128u) * (left > kTK ? kSub : 1));
+          for (int sub = 0; sub < kSub; ++sub, st += kSubBytes) {
+            if (sub * kTK >= left) break;
+            const int k = k0 + sub * kTK;
+            if (warp == 0) {
+              if (KIND == kGroupedFwd) {
+                tma::load_3d(st, &maps.p[0], bar, k * 2, m0, it.e);
+              } else if (KIND == kGroupedDgrad) {
+                tma::load_3d(st, &maps.p[0], bar, m0 * 2, k, it.e);
+                tma::load_3d(st + kMnBox, &maps.p[0], bar, m0 * 2 + 128, k, it.e);
+              } else {
+                load_mn(st, maps.p, bar, m0, 2, it.row0 + k, left - sub * kTK, a.R);
+              }
             } else {
-              load_mn(st, maps.p, bar, m0, 2, kr, left, a.R);
-            }
-          } else {
-            st += kABytes;
-            if (kQMn) {
-              load_mn(st, maps.q, bar, c0, boxes, kr, left, a.R);
-            } else {
-              if (half & 192) tma::load_3d(st, &maps.q[0], bar, kb * 128, c0, 0);
-              if (half & 128) tma::load_3d(st + 64 * 128, &maps.q[0], bar, kb * 128, c0 + 64, 0);
-              if (half & 32)
-                tma::load_3d(st + (half & 64) * 128, &maps.q[1], bar, kb * 128, c0 + (half & 64), 0);
-              if (half & 16)
-                tma::load_3d(st + (half & 96) * 128, &maps.q[2], bar, kb * 128, c0 + (half & 96), 0);
+              uint8_t *sq = st + kABytes;
+              if (kQMn) {
+                load_mn(sq, maps.q, bar, c0, boxes, it.row0 + k, left - sub * kTK, a.R);
+              } else {
+                if (half & 192) tma::load_3d(sq, &maps.q[0], bar, k * 2, c0, 0);
+                if (half & 128) tma::load_3d(sq + 64 * 128, &maps.q[0], bar, k * 2, c0 + 64, 0);
+                if (half & 32)
+                  tma::load_3d(sq + (half & 64) * 128, &maps.q[1], bar, k * 2, c0 + (half & 64), 0);
+                if (half & 16)
+                  tma::load_3d(sq + (half & 96) * 128, &maps.q[2], bar, k * 2, c0 + (half & 96), 0);
+              }
             }
           }
         }
         __syncwarp();
       }
     }
-    if (!ok) pp.drain(q);
+    if (!ok) pp.drain(ring);
   } else if (warp == 1) {
     // fp32 sums, both operands of one type, M = 256
     const uint32_t fmt = a.dtype == MOE_DT_BF16 ? 1u : 0u;
     const uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)kPMn << 15) |
                             ((uint32_t)kQMn << 16) | ((uint32_t)(kTM >> 4) << 24);
-    int q = 0, j = 0;
+    // 16 elements of K further: 32 bytes of a row, or 16 rows of 128 bytes
+    constexpr uint64_t kPStep = (kPMn ? 2048 : 32) >> 4, kQStep = (kQMn ? 2048 : 32) >> 4;
+    const uint64_t pd0 = sw128_desc(su32(tiles), kPMn ? kMnBox : 16, 1024);
+    const uint64_t qd0 = sw128_desc(su32(tiles) + kABytes, kQMn ? kMnBox : 16, 1024);
+    Ring<kStages> ring;
+    int j = 0;
     for (int w = pair; w < work.total; w += pairs) {
       const Item it = work.item(w);
-      const int nk = (it.len + kTK - 1) / kTK;
-      if (nk == 0) continue;
+      if (it.len == 0) continue;
       const int buf = j & 1;
       if (rank == 0 && j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
-      fence_after_sync();
       const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 31) >> 5) << 19);
       bool ok = true;
-      for (int kb = 0; kb < nk; ++kb, ++q) {
-        const int s = q % kStages;
-        if (!pp.wait_warp(&pp.full[s], (q / kStages) & 1)) {
+      for (int k0 = 0; k0 < it.len; k0 += kSub * kTK, ring.next()) {
+        if (!pp.wait_warp(&pp.full[ring.s], ring.use & 1)) {
           ok = false;
           break;
         }
-        uint8_t *st = tiles + s * kStageBytes;
-        const int steps = kQMn ? min(kTK, it.len - kb * kTK + 15) / 16 : kTK / 16;
         fence_after_sync();
         if (rank != 0) {
-          if (elect_one()) arrive_at(&pp.full[s], 0);
+          if (elect_one()) arrive_at(&pp.full[ring.s], 0);
         } else if (elect_one()) {
-          const uint32_t base = su32(st);
-          const uint64_t pd = kPMn ? sw128_desc(base, kMnBox, 1024) : sw128_desc(base, 16, 1024);
-          const uint64_t qd = kQMn ? sw128_desc(base + kABytes, kMnBox, 1024)
-                                   : sw128_desc(base + kABytes, 16, 1024);
-          // 16 elements of K further: 32 bytes of a row, or 16 rows of 128 bytes
-          constexpr uint64_t kPStep = (kPMn ? 2048 : 32) >> 4, kQStep = (kQMn ? 2048 : 32) >> 4;
-          if (steps == kTK / 16) {
+          const uint64_t at = (uint64_t)(ring.s * (kStageBytes >> 4));
+          const int left = it.len - k0;
+          if (left >= kSub * kTK || (!kQMn && left > kTK)) {
 #pragma unroll
-            for (int k = 0; k < kTK / 16; ++k)
-              mma_f16_pair(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < kSub * kTK / 16; ++k) {
+              const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (kSubBytes >> 4);
+              mma_f16_pair(d, pd0 + sub + k % (kTK / 16) * kPStep,
+                           qd0 + sub + k % (kTK / 16) * kQStep, idesc, (k0 > 0 || k > 0) ? 1u : 0u);
+            }
           } else {
-            for (int k = 0; k < steps; ++k)
-              mma_f16_pair(d, pd + k * kPStep, qd + k * kQStep, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            // forward and dgrad: one block of kTK, the rest of it zeros; wgrad: the
+            // rows there are, in steps of 16
+            const int steps = kQMn ? (left + 15) / 16 : kTK / 16;
+            for (int k = 0; k < steps; ++k) {
+              const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (kSubBytes >> 4);
+              mma_f16_pair(d, pd0 + sub + k % (kTK / 16) * kPStep,
+                           qd0 + sub + k % (kTK / 16) * kQStep, idesc, (k0 > 0 || k > 0) ? 1u : 0u);
+            }
           }
-          commit_pair(&pp.empty[s]);
+          commit_pair(&pp.empty[ring.s]);
         }
         __syncwarp();
       }

@@ -12,11 +12,16 @@
 // 2i of a row in the low nibble; scales [rows][4 ceil(k / 128)], the bytes
 // behind the last block zero; values behind k are zeros.
 //
-// Both directions move each byte once and are bound by HBM.  A warp takes
-// 256 values of a row (8 a lane, one 16-byte load of 16-bit values): a block
-// is 4 lanes, its maximum two shuffles, and a lane stores its 8 codes as one
-// word, so a warp's store is 128 contiguous bytes.
+// Both directions move each byte once and are bound by HBM, with the issue slots
+// close behind, so 16-bit values stay packed: the maximum of a block is taken
+// on pairs of magnitudes, and codes become bf16 by byte lookups (prmt) and one
+// packed multiplication by the scale.  A warp takes 256 values of a row at a
+// time (8 a lane, one 16-byte load of 16-bit values), four such spans in
+// flight: a block is 4 lanes, its maximum two shuffles, and a lane stores its 8
+// codes as one word, so a warp's store is 128 contiguous bytes.  Rows go to
+// warps, or their parts to several (a power of two) where rows are few.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/moe_b200.h"
 #include "common.cuh"
@@ -26,7 +31,8 @@
 namespace moe {
 namespace {
 
-constexpr int kQThreads = 256, kSpan = 256;  // values of a warp's unit
+constexpr int kQThreads = 256, kSpan = 256;  // values of a warp's step
+constexpr int kFlight = 4;                   // spans whose loads are issued together
 
 // Codes of eight values already divided by the scale, value i in nibble i.
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
@@ -42,113 +48,206 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   return r;
 }
 
-// The value of E2M1 code c, exactly.
-__device__ __forceinline__ float e2m1_value(uint32_t c) {
-  const uint32_t m = c & 7u;
-  // m = 1 is 0.5; from 2 on, exponent m >> 1 and one fraction bit, as in fp32
-  const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-  return (c & 8u) ? -v : v;
-}
+// Eight values of a row as they lie in memory; for fp32 as their bits.
+template <typename T>
+struct Raw8 {
+  uint32_t w[2 * sizeof(T)];
 
-__device__ __forceinline__ float e8m0_value(uint32_t b) {
-  if (b == 255u) return __uint_as_float(0x7fffffffu);
-  return __uint_as_float(b ? b << 23 : 1u << 22);
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_span(const T *row, int c, int k, float (&v)[8]) {
-  if (VEC && c + 8 <= k) {
-    load8(row + c, v);
-  } else {
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T *row, int c, int k) {
+    if (VEC && c + 8 <= k) {
+      const uint4 *p = reinterpret_cast<const uint4 *>(row + c);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < k ? to_f32(row[c + i]) : 0.0f;
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) *reinterpret_cast<uint4 *>(w + 4 * i) = __ldg(p + i);
+    } else {
+      T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = c + i < k ? row[c + i] : T(0.0f);
+    }
   }
-}
+  __device__ __forceinline__ float value(int i) const {
+    return to_f32(reinterpret_cast<const T *>(w)[i]);
+  }
+  // The fp32 bits of the largest magnitude; any NaN counts above infinity.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t m =
+          __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                   __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+      const unsigned short h = (unsigned short)max(m & 0xffffu, m >> 16);
+      return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    }
+  }
+};
+
+// A warp's rows and spans: parts = 1 << shift warps share a row.
+struct SpanWalk {
+  int lane, part, parts;
+  long long row, step;
+  __device__ __forceinline__ explicit SpanWalk(int shift) {
+    const long long w = (long long)blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5);
+    lane = threadIdx.x & 31;
+    parts = 1 << shift;
+    part = (int)(w & (parts - 1));
+    row = w >> shift;
+    step = ((long long)gridDim.x * (kQThreads / 32)) >> shift;
+  }
+};
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQThreads) mxfp4_quantize_kernel(Mxfp4Quant a) {
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kQThreads) mxfp4_quantize_kernel(Mxfp4Quant a, int shift) {
+  const SpanWalk sw(shift);
   const int spans = (a.k + kSpan - 1) / kSpan, nb = (a.k + 31) / 32;
   const int ldc = mxfp4_code_stride(a.k), lds = mxfp4_scale_stride(a.k);
-  const long long units = (long long)a.rows * spans;
-  const long long step = (long long)gridDim.x * (kQThreads / 32);
-  for (long long u = (long long)blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); u < units;
-       u += step) {
-    const int r = (int)(u / spans), c = (int)(u % spans) * kSpan + lane * 8, blk = c / 32;
-    int src = r;
+  for (long long r = sw.row; r < a.rows; r += sw.step) {
+    long long src = r;
     if (a.index) {
       src = a.index[r];
       if (src < 0 || src >= a.src_rows) {
-        if (lane == 0) set_status(a.status, kStatusBadRoute);
+        if (sw.lane == 0) set_status(a.status, kStatusBadRoute);
         src = -1;
       }
     }
-    float v[8] = {};
-    if (src >= 0) load_span<T, VEC>(reinterpret_cast<const T *>(a.x) + src * a.ld_x, c, a.k, v);
-    // as integers, |NaN| > infinity > every finite |v|
-    uint32_t m = 0;
+    const T *row = reinterpret_cast<const T *>(a.x) + src * a.ld_x;
+    for (int s0 = sw.part; s0 < spans; s0 += kFlight * sw.parts) {
+      Raw8<T> x[kFlight];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t ex = m >> 23;  // floor(log2 max) + 127 (0 for subnormal numbers)
-    const uint32_t sb = ex == 255u ? 255u : (ex > 2u ? ex - 2u : 0u);
-    const float inv = __uint_as_float((254u - min(sb, 252u)) << 23);  // 2^(127 - sb), normal
+      for (int f = 0; f < kFlight; ++f)
+        x[f].template load<VEC>(row, (s0 + f * sw.parts) * kSpan + sw.lane * 8, src < 0 ? 0 : a.k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ex == 255u ? 0.0f : v[i] * inv;
-    const uint32_t q = e2m1x8(v);
-    if (blk < nb) *reinterpret_cast<uint32_t *>(a.codes + (int64_t)r * ldc + c / 2) = q;
-    if ((lane & 3) == 0 && blk < lds) a.scales[(int64_t)r * lds + blk] = blk < nb ? sb : 0;
+      for (int f = 0; f < kFlight; ++f) {
+        const int c = (s0 + f * sw.parts) * kSpan + sw.lane * 8, blk = c / 32;
+        if (s0 + f * sw.parts >= spans) break;  // warp-uniform
+        uint32_t m = x[f].top();
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const uint32_t ex = m >> 23;  // floor(log2 max) + 127 (0 for subnormal numbers)
+        const uint32_t sb = ex == 255u ? 255u : (ex > 2u ? ex - 2u : 0u);
+        const float inv = __uint_as_float((254u - min(sb, 252u)) << 23);  // 2^(127 - sb), normal
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[f].value(i) * inv;
+        const uint32_t q = ex == 255u ? 0u : e2m1x8(v);
+        if (blk < nb) *reinterpret_cast<uint32_t *>(a.codes + r * ldc + c / 2) = q;
+        // a warp's span has 8 scales; two lanes store 4 of them each
+        uint32_t word = blk < nb ? sb << (sw.lane / 4 % 4 * 8) : 0u;
+        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+        if (sw.lane % 16 == 0 && blk < lds)
+          *reinterpret_cast<uint32_t *>(a.scales + r * lds + blk) = word;
+      }
+    }
+  }
+}
+
+// The bf16 of the eight codes in q, codes 2i and 2i + 1 in word i: the bytes of
+// 0 0.5 1 1.5 2 3 4 6 are looked up by the codes' low three bits.
+__device__ __forceinline__ void e2m1x8_bf16(uint32_t q, uint32_t (&w)[4]) {
+  const uint32_t sel = q & 0x77777777u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t s = sel >> (16 * h);
+    const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, s);
+    const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, s);
+    const uint32_t sg = q >> (16 * h);
+    w[2 * h] = __byte_perm(lo, hi, 0x5140) | (sg & 8u) << 12 | (sg & 0x80u) << 24;
+    w[2 * h + 1] = __byte_perm(lo, hi, 0x7362) | (sg & 0x800u) << 4 | (sg & 0x8000u) << 16;
   }
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQThreads) mxfp4_dequantize_kernel(Mxfp4Dequant a) {
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kQThreads) mxfp4_dequantize_kernel(Mxfp4Dequant a, int shift) {
+  const SpanWalk sw(shift);
   const int spans = (a.k + kSpan - 1) / kSpan;
   const int ldc = mxfp4_code_stride(a.k), lds = mxfp4_scale_stride(a.k);
-  const long long units = (long long)a.rows * spans;
-  const long long step = (long long)gridDim.x * (kQThreads / 32);
-  for (long long u = (long long)blockIdx.x * (kQThreads / 32) + (threadIdx.x >> 5); u < units;
-       u += step) {
-    const int64_t r = u / spans;
-    const int c = (int)(u % spans) * kSpan + lane * 8;
-    if (c >= a.k) continue;
-    const uint32_t q = *reinterpret_cast<const uint32_t *>(a.codes + r * ldc + c / 2);
-    const float s = e8m0_value(a.scales[r * lds + c / 32]);
-    float v[8];
+  for (long long r = sw.row; r < a.rows; r += sw.step) {
+    const uint8_t *codes = a.codes + r * ldc, *scales = a.scales + r * lds;
+    T *row = reinterpret_cast<T *>(a.out) + r * a.ld_out;
+    for (int s0 = sw.part; s0 < spans; s0 += kFlight * sw.parts) {
+      uint32_t q[kFlight], sb[kFlight];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = e2m1_value(q >> (4 * i) & 15u) * s;
-    T *o = reinterpret_cast<T *>(a.out) + r * a.ld_out + c;
-    if (VEC && c + 8 <= a.k) {
-      store8(o, v);
-    } else {
-      for (int i = 0; i < 8 && c + i < a.k; ++i) o[i] = from_f32<T>(v[i]);
+      for (int f = 0; f < kFlight; ++f) {
+        const int c = (s0 + f * sw.parts) * kSpan + sw.lane * 8;
+        q[f] = c < a.k ? __ldg(reinterpret_cast<const uint32_t *>(codes + c / 2)) : 0u;
+        sb[f] = c < a.k ? __ldg(scales + c / 32) : 0u;
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        const int c = (s0 + f * sw.parts) * kSpan + sw.lane * 8;
+        if (c >= a.k) break;
+        uint32_t w[4];
+        e2m1x8_bf16(q[f], w);
+        // 2^(sb - 127) as a bf16: exponent bits, the subnormal 2^-127, or NaN
+        const uint32_t sc = sb[f] == 255u ? 0x7fffu : sb[f] ? sb[f] << 7 : 0x40u;
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+          const uint32_t s2 = sc | sc << 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 p = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&w[i]),
+                                             *reinterpret_cast<const __nv_bfloat162 *>(&s2));
+            w[i] = *reinterpret_cast<const uint32_t *>(&p);
+          }
+          if (VEC && c + 8 <= a.k) {
+            *reinterpret_cast<uint4 *>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+            for (int i = 0; i < 8 && c + i < a.k; ++i)
+              row[c + i] = reinterpret_cast<const __nv_bfloat16 *>(w)[i];
+          }
+        } else {
+          const float s = __uint_as_float(sc << 16);
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16) * s;
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * s;
+          }
+          if (VEC && c + 8 <= a.k) {
+            store8(row + c, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < a.k) row[c + i] = from_f32<T>(v[i]);
+          }
+        }
+      }
     }
   }
 }
 
-int span_grid(int rows, int k, int sm_count) {
-  const long long units = (long long)rows * ((k + kSpan - 1) / kSpan);
-  return (int)std::min<long long>((units + kQThreads / 32 - 1) / (kQThreads / 32),
-                                  (long long)sm_count * 8);
+// Warps of a row, as a shift: 1, or a power of two up to its spans while the
+// rows alone would leave the GPU's warps idle; and the grid.
+int row_split(int rows, int k, int sm_count, int *grid) {
+  const long long warps = (long long)sm_count * 8 * (kQThreads / 32);
+  const int spans = (k + kSpan - 1) / kSpan;
+  int shift = 0;
+  while ((2 << shift) <= spans && ((long long)rows << (shift + 1)) <= warps) ++shift;
+  const long long blocks = (((long long)rows << shift) + kQThreads / 32 - 1) / (kQThreads / 32);
+  *grid = (int)std::min<long long>(blocks, (long long)sm_count * 8);
+  return shift;
 }
 
 template <typename T>
 cudaError_t quantize_t(const Mxfp4Quant &a, cudaStream_t s) {
   const bool vec = ((uintptr_t)a.x & 15) == 0 && (a.ld_x * sizeof(T)) % 16 == 0;
-  const int grid = span_grid(a.rows, a.k, a.sm_count);
-  if (vec) mxfp4_quantize_kernel<T, true><<<grid, kQThreads, 0, s>>>(a);
-  else mxfp4_quantize_kernel<T, false><<<grid, kQThreads, 0, s>>>(a);
+  int grid;
+  const int shift = row_split(a.rows, a.k, a.sm_count, &grid);
+  if (vec) mxfp4_quantize_kernel<T, true><<<grid, kQThreads, 0, s>>>(a, shift);
+  else mxfp4_quantize_kernel<T, false><<<grid, kQThreads, 0, s>>>(a, shift);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t dequantize_t(const Mxfp4Dequant &a, cudaStream_t s) {
   const bool vec = ((uintptr_t)a.out & 15) == 0 && (a.ld_out * sizeof(T)) % 16 == 0;
-  const int grid = span_grid(a.rows, a.k, a.sm_count);
-  if (vec) mxfp4_dequantize_kernel<T, true><<<grid, kQThreads, 0, s>>>(a);
-  else mxfp4_dequantize_kernel<T, false><<<grid, kQThreads, 0, s>>>(a);
+  int grid;
+  const int shift = row_split(a.rows, a.k, a.sm_count, &grid);
+  if (vec) mxfp4_dequantize_kernel<T, true><<<grid, kQThreads, 0, s>>>(a, shift);
+  else mxfp4_dequantize_kernel<T, false><<<grid, kQThreads, 0, s>>>(a, shift);
   return cudaGetLastError();
 }
 

@@ -82,14 +82,14 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   };
 
   if (warp == 0 || warp == 2) {
-    int q = 0;
+    Ring<kStages> ring;
     bool ok = true;
     for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
       const Item it = item(w);
       const int rows = (it.nc + 15) & ~15;
-      for (int kb = 0; kb < nk; ++kb, ++q) {
-        const int s = q % kStages, use = q / kStages;
-        ok = use == 0 || pp.wait_warp(&pp.empty[s], (use - 1) & 1);
+      for (int kb = 0; kb < nk; ++kb, ring.next()) {
+        const int s = ring.s;
+        ok = ring.use == 0 || pp.wait_warp(&pp.empty[s], (ring.use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
           uint8_t *st = tiles + s * kStageBytes;
@@ -112,12 +112,13 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         __syncwarp();
       }
     }
-    if (!ok) pp.drain(q);
+    if (!ok) pp.drain(ring);
   } else if (warp == 1) {
     // E2M1 operands, E8M0 scales, M = 128
     const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kTM >> 4) << 24);
     const uint32_t sf0 = pp.tmem_base + 2 * kTN;
-    int q = 0, j = 0;
+    Ring<kStages> ring;
+    int j = 0;
     for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
       const int buf = j & 1;
@@ -126,9 +127,9 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 15) >> 4) << 18);
       bool ok = true;
-      for (int kb = 0; kb < nk; ++kb, ++q) {
-        const int s = q % kStages;
-        if (!pp.wait_warp(&pp.full[s], (q / kStages) & 1)) {
+      for (int kb = 0; kb < nk; ++kb, ring.next()) {
+        const int s = ring.s;
+        if (!pp.wait_warp(&pp.full[s], ring.use & 1)) {
           ok = false;
           break;
         }

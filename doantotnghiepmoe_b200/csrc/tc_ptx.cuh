@@ -117,6 +117,19 @@ __device__ __forceinline__ uint64_t rows16_desc(uint32_t saddr) {
 constexpr int kEpiWarps = 16;  // four a TMEM lane quarter
 constexpr int kThreads = 96 + 32 * kEpiWarps;
 
+// A position in a ring of S stages: the stage and the parity of its use.
+template <int S>
+struct Ring {
+  int s = 0;
+  uint32_t use = 0;  // how often the ring went round
+  __device__ __forceinline__ void next() {
+    if (++s == S) {
+      s = 0;
+      ++use;
+    }
+  }
+};
+
 template <int S>
 struct Pipe {
   uint64_t full[S], empty[S];  // stages of the shared-memory ring
@@ -138,11 +151,13 @@ struct Pipe {
     abort_flag = 0;
     tma::fence_mbar_init();
   }
-  // After q issued stages and an abort: the copies in flight land before the
-  // CTA may exit (a bounded wait for the last use of each stage).
-  __device__ __forceinline__ void drain(int q) {
-    for (int k = max(q - S, 0); k < q; ++k)
-      tma::mbar_wait(&full[k % S], (k / S) & 1, nullptr, tma::kWaitCycles / 64);
+  // After an abort: the copies in flight land before the CTA may exit (a bounded
+  // wait for the last use of each stage).
+  __device__ __forceinline__ void drain(const Ring<S> &r) {
+    for (int s = 0; s < S; ++s) {
+      const uint32_t uses = r.use + (s < r.s ? 1 : 0);
+      if (uses) tma::mbar_wait(&full[s], (uses - 1) & 1, nullptr, tma::kWaitCycles / 64);
+    }
   }
   // A whole warp's bounded wait; false (for every lane) once any role gave up.
   __device__ __forceinline__ bool wait_warp(uint64_t *bar, uint32_t parity) {
