@@ -56,23 +56,22 @@ __device__ __forceinline__ void block_sums(float (&v)[N], float (*buf)[kMaxThrea
   }
 }
 
-// Values (n * blockDim + thread) * V .. + V - 1 of a row.
-template <typename T, int V>
-__device__ __forceinline__ void load_v(const T *p, int c, int H, float (&v)[V]) {
-  if constexpr (V == 8) {
-    if (c < H) load8(p + c, v);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-  } else {
-    v[0] = c < H ? to_f32(p[c]) : 0.0f;
-  }
-}
 template <typename T, int V>
 __device__ __forceinline__ void store_v(T *p, int c, int H, const float (&v)[V]) {
   if (c >= H) return;
   if constexpr (V == 8) store8(p + c, v);
   else p[c] = from_f32<T>(v[0]);
+}
+
+// A gain's values, or ones.
+template <int V>
+__device__ __forceinline__ void load_gain(Piece<float, V> &w, const float *g, int c, int H) {
+  if (g) {
+    w.load(g, c, H);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w.w[i] = __float_as_uint(1.0f);
+  }
 }
 
 template <typename TX, typename TY, int V, int NE>
@@ -82,66 +81,71 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(BlockNormArgs a
   const int64_t r = blockIdx.x;
   const int H = a.H;
   const float inv_h = 1.0f / (float)H;
-  const TX *x = reinterpret_cast<const TX *>(a.x) + r * a.ld_res;
-  float xo[NE][V];
-#pragma unroll
-  for (int n = 0; n < NE; ++n) load_v<TX, V>(x, (n * blockDim.x + threadIdx.x) * V, H, xo[n]);
-#pragma unroll
-  for (int n = 0; n < NE; ++n)
-#pragma unroll
-    for (int i = 0; i < V; ++i) xo[n][i] *= a.scale;
-  if (a.y) {
-    const TY *y = reinterpret_cast<const TY *>(a.y) + r * a.ld_blk;
-    float yv[NE][V];
-#pragma unroll
-    for (int n = 0; n < NE; ++n) load_v<TY, V>(y, (n * blockDim.x + threadIdx.x) * V, H, yv[n]);
-    float g = a.gate ? a.gate[r] : 1.0f;
-    if (a.post) {
-      float s[1] = {0.0f};
-#pragma unroll
-      for (int n = 0; n < NE; ++n)
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[0] = fmaf(yv[n][i], yv[n][i], s[0]);
-      block_sums(s, buf, flip);
-      g *= __frsqrt_rn(s[0] * inv_h + a.eps);
-    }
-#pragma unroll
-    for (int n = 0; n < NE; ++n) {
-      const int c = (n * blockDim.x + threadIdx.x) * V;
-      float w[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = 1.0f;
-      if (a.post && a.w_post) load_v<float, V>(a.w_post, c, H, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) xo[n][i] = fmaf(g * w[i], yv[n][i], xo[n][i]);
-    }
-  }
-  if (a.x_out) {
-    TX *o = reinterpret_cast<TX *>(a.x_out) + r * a.ld_res;
-#pragma unroll
-    for (int n = 0; n < NE; ++n) store_v<TX, V>(o, (n * blockDim.x + threadIdx.x) * V, H, xo[n]);
-  }
-  if (!a.h) return;
-  float s[1] = {0.0f};
-#pragma unroll
-  for (int n = 0; n < NE; ++n)
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[0] = fmaf(xo[n][i], xo[n][i], s[0]);
-  block_sums(s, buf, flip);
-  const float rq = __frsqrt_rn(s[0] * inv_h + a.eps);
-  TY *h = reinterpret_cast<TY *>(a.h) + r * a.ld_blk;
+  const bool post = a.y && a.post;
+  // everything a row needs is on its way before the first sum
+  Piece<TX, V> x[NE];
+  Piece<TY, V> y[NE];
+  Piece<float, V> wq[NE], wp[NE];
 #pragma unroll
   for (int n = 0; n < NE; ++n) {
     const int c = (n * blockDim.x + threadIdx.x) * V;
-    float w[V];
+    if (a.y) y[n].load(reinterpret_cast<const TY *>(a.y) + r * a.ld_blk, c, H);
+    else y[n].clear();
+    x[n].load(reinterpret_cast<const TX *>(a.x) + r * a.ld_res, c, H);
+    load_gain<V>(wp[n], post ? a.w_post : nullptr, c, H);
+    load_gain<V>(wq[n], a.w_pre, c, H);
+  }
+  float g = a.y && a.gate ? a.gate[r] : 1.0f;
+  if (post) {
+    float s[1] = {0.0f};
 #pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = 1.0f;
-    if (a.w_pre) load_v<float, V>(a.w_pre, c, H, w);
+    for (int n = 0; n < NE; ++n)
 #pragma unroll
-    for (int i = 0; i < V; ++i) w[i] *= xo[n][i] * rq;
-    store_v<TY, V>(h, c, H, w);
+      for (int i = 0; i < V; ++i) s[0] = fmaf(y[n][i], y[n][i], s[0]);
+    block_sums(s, buf, flip);
+    g *= __frsqrt_rn(s[0] * inv_h + a.eps);
+  }
+  float xo[NE][V], s[1] = {0.0f};
+#pragma unroll
+  for (int n = 0; n < NE; ++n) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      xo[n][i] = x[n][i] * a.scale;
+      if (a.y) xo[n][i] = fmaf(g * wp[n][i], y[n][i], xo[n][i]);
+      s[0] = fmaf(xo[n][i], xo[n][i], s[0]);
+    }
+    if (a.x_out)
+      store_v<TX, V>(reinterpret_cast<TX *>(a.x_out) + r * a.ld_res,
+                     (n * blockDim.x + threadIdx.x) * V, H, xo[n]);
+  }
+  if (!a.h) return;
+  block_sums(s, buf, flip);
+  const float rq = __frsqrt_rn(s[0] * inv_h + a.eps);
+#pragma unroll
+  for (int n = 0; n < NE; ++n) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) xo[n][i] *= rq * wq[n][i];
+    store_v<TY, V>(reinterpret_cast<TY *>(a.h) + r * a.ld_blk,
+                   (n * blockDim.x + threadIdx.x) * V, H, xo[n]);
   }
 }
+
+// What the backward pass reads of a row.
+template <typename TX, typename TY, int V>
+struct BwdRow {
+  Piece<TX, V> x, d;
+  Piece<TY, V> c, y;
+  __device__ __forceinline__ void load(const BlockNormArgs &a, int64_t r, int at) {
+    const int H = r < a.rows ? a.H : 0;
+    x.load(reinterpret_cast<const TX *>(a.x) + r * a.ld_res, at, H);
+    if (a.dx_out) d.load(reinterpret_cast<const TX *>(a.dx_out) + r * a.ld_res, at, H);
+    else d.clear();
+    if (a.dh) c.load(reinterpret_cast<const TY *>(a.dh) + r * a.ld_blk, at, H);
+    else c.clear();
+    if (a.y) y.load(reinterpret_cast<const TY *>(a.y) + r * a.ld_blk, at, H);
+    else y.clear();
+  }
+};
 
 template <typename TX, typename TY, int V, int NE>
 __global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(BlockNormArgs a) {
@@ -149,80 +153,78 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(BlockNormAr
   int flip = 0;
   const int H = a.H;
   const float inv_h = 1.0f / (float)H;
+  const bool post = a.y && a.post;
+  // The next row is loaded before this one's sums where its registers allow.
+  constexpr bool kAhead = V * NE <= 8;
   float wpre[NE][V] = {}, wpost[NE][V] = {};  // sums of the gains' gradients
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    float x[NE][V], d[NE][V], y[NE][V] = {}, c[NE][V] = {};
-    const TX *xp = reinterpret_cast<const TX *>(a.x) + r * a.ld_res;
+  Piece<float, V> gq[NE], gp[NE];
+  BwdRow<TX, TY, V> next[NE];
 #pragma unroll
-    for (int n = 0; n < NE; ++n) {
-      const int at = (n * blockDim.x + threadIdx.x) * V;
-      load_v<TX, V>(xp, at, H, x[n]);
-      if (a.dx_out)
-        load_v<TX, V>(reinterpret_cast<const TX *>(a.dx_out) + r * a.ld_res, at, H, d[n]);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) d[n][i] = 0.0f;
-      if (a.dh) load_v<TY, V>(reinterpret_cast<const TY *>(a.dh) + r * a.ld_blk, at, H, c[n]);
-      if (a.y) load_v<TY, V>(reinterpret_cast<const TY *>(a.y) + r * a.ld_blk, at, H, y[n]);
+  for (int n = 0; n < NE; ++n) {
+    const int at = (n * blockDim.x + threadIdx.x) * V;
+    if (kAhead) {
+      load_gain<V>(gq[n], a.w_pre, at, H);
+      load_gain<V>(gp[n], post ? a.w_post : nullptr, at, H);
+      next[n].load(a, blockIdx.x, at);
     }
+  }
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    BwdRow<TX, TY, V> row[NE];
     float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
-      float w[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = 1.0f;
-      if (a.w_pre) load_v<float, V>(a.w_pre, (n * blockDim.x + threadIdx.x) * V, H, w);
+      const int at = (n * blockDim.x + threadIdx.x) * V;
+      if (kAhead) {
+        row[n] = next[n];
+        next[n].load(a, r + gridDim.x, at);
+      } else {
+        row[n].load(a, r, at);
+        load_gain<V>(gq[n], a.w_pre, at, H);
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[0] = fmaf(x[n][i], x[n][i], s[0]);
-        s[1] = fmaf(c[n][i] * w[i], x[n][i], s[1]);
-        s[2] = fmaf(y[n][i], y[n][i], s[2]);
+        s[0] = fmaf(row[n].x[i], row[n].x[i], s[0]);
+        s[1] = fmaf(row[n].c[i] * gq[n][i], row[n].x[i], s[1]);
+        s[2] = fmaf(row[n].y[i], row[n].y[i], s[2]);
       }
     }
     block_sums(s, buf, flip);
     const float rq = a.dh ? __frsqrt_rn(s[0] * inv_h + a.eps) : 0.0f;
-    const float rp = a.post ? __frsqrt_rn(s[2] * inv_h + a.eps) : 1.0f;
+    const float rp = post ? __frsqrt_rn(s[2] * inv_h + a.eps) : 1.0f;
     const float kx = rq * rq * rq * s[1] * inv_h;
-    const float g = a.gate ? a.gate[r] : 1.0f;
-    float t[1] = {0.0f};
+    const float g = a.y && a.gate ? a.gate[r] : 1.0f;
+    float t[1] = {0.0f}, d[NE][V];
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
       const int at = (n * blockDim.x + threadIdx.x) * V;
-      float w[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = 1.0f;
-      if (a.w_pre) load_v<float, V>(a.w_pre, at, H, w);
+      if (!kAhead) {
+        load_gain<V>(gq[n], a.w_pre, at, H);
+        load_gain<V>(gp[n], post ? a.w_post : nullptr, at, H);
+      }
+      float o[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        wpre[n][i] = fmaf(c[n][i], x[n][i] * rq, wpre[n][i]);
-        d[n][i] = fmaf(rq, c[n][i] * w[i], d[n][i]) - kx * x[n][i];
-        w[i] = a.scale * d[n][i];
+        const float x = row[n].x[i], c = row[n].c[i];
+        wpre[n][i] = fmaf(c, x * rq, wpre[n][i]);
+        d[n][i] = fmaf(rq, c * gq[n][i], row[n].d[i]) - kx * x;
+        o[i] = a.scale * d[n][i];
+        wpost[n][i] = fmaf(g * d[n][i], row[n].y[i] * rp, wpost[n][i]);
+        d[n][i] *= gp[n][i];
+        t[0] = fmaf(d[n][i], row[n].y[i], t[0]);
       }
-      store_v<TX, V>(reinterpret_cast<TX *>(a.dx) + r * a.ld_res, at, H, w);
-      if (!a.y) continue;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        wpost[n][i] = fmaf(g * d[n][i], y[n][i] * rp, wpost[n][i]);
-        w[i] = 1.0f;
-      }
-      if (a.post && a.w_post) load_v<float, V>(a.w_post, at, H, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        d[n][i] *= w[i];
-        t[0] = fmaf(d[n][i], y[n][i], t[0]);
-      }
+      store_v<TX, V>(reinterpret_cast<TX *>(a.dx) + r * a.ld_res, at, H, o);
     }
     if (!a.y) continue;
     float ky = 0.0f;
-    if (a.post || a.dgate) {
+    if (post || a.dgate) {
       block_sums(t, buf, flip);
-      if (a.post) ky = rp * rp * t[0] * inv_h;
+      if (post) ky = rp * rp * t[0] * inv_h;
       if (a.dgate && threadIdx.x == 0) a.dgate[r] = rp * t[0];
     }
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[n][i] = g * rp * (d[n][i] - ky * y[n][i]);
+      for (int i = 0; i < V; ++i) d[n][i] = g * rp * (d[n][i] - ky * row[n].y[i]);
       store_v<TY, V>(reinterpret_cast<TY *>(a.dy) + r * a.ld_blk,
                      (n * blockDim.x + threadIdx.x) * V, H, d[n]);
     }
@@ -240,20 +242,22 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(BlockNormAr
     }
 }
 
-// dw[c] = the sum over the CTAs' partial sums, in the order of the CTAs: 8
-// interleaved chains a column, joined in a fixed order.
-__global__ void __launch_bounds__(256) block_norm_gains_kernel(const float *part, int ctas, int H,
-                                                               float *dw_pre, float *dw_post) {
-  __shared__ float sm[8][33];
+// dw[c] = the sum over the CTAs' partial sums, in an order that their number
+// fixes: a warp a chain of every 32nd, then the chains one after another.
+__global__ void __launch_bounds__(1024) block_norm_gains_kernel(const float *part, int ctas, int H,
+                                                                float *dw_pre, float *dw_post) {
+  __shared__ float sm[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.0f;
-  if (c < 2 * H)
-    for (int g = w; g < ctas; g += 8) s += part[(int64_t)g * 2 * H + c];
+  if (c < 2 * H) {
+#pragma unroll 4
+    for (int g = w; g < ctas; g += 32) s += part[(int64_t)g * 2 * H + c];
+  }
   sm[w][lane] = s;
   __syncthreads();
   if (w || c >= 2 * H) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += sm[i][lane];
+  for (int i = 1; i < 32; ++i) s += sm[i][lane];
   if (c < H) {
     if (dw_pre) dw_pre[c] = s;
   } else if (dw_post) {
@@ -308,7 +312,7 @@ bool vec_ok(const BlockNormArgs &a) {
 
 int block_norm_backward_ctas(int rows, int H, int sm_count) {
   (void)H;
-  return std::max(1, std::min(rows, sm_count * 4));
+  return std::max(1, std::min(rows, sm_count * 3));
 }
 
 cudaError_t launch_block_norm(const BlockNormArgs &a, cudaStream_t s) {
@@ -334,7 +338,7 @@ cudaError_t launch_block_norm_backward(const BlockNormArgs &a, cudaStream_t s) {
     });
   });
   if (e != cudaSuccess || (!a.dw_pre && !a.dw_post)) return e;
-  block_norm_gains_kernel<<<(2 * a.H + 31) / 32, 256, 0, s>>>(a.partial, ctas, a.H, a.dw_pre,
+  block_norm_gains_kernel<<<(2 * a.H + 31) / 32, 1024, 0, s>>>(a.partial, ctas, a.H, a.dw_pre,
                                                              a.dw_post);
   return cudaGetLastError();
 }

@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace moe {
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -18,6 +20,39 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
+
+// V = 8 or 1 elements of a row, as they lie in memory: what a thread holds of a
+// row that is still on its way.
+template <typename T, int V>
+struct Piece {
+  uint32_t w[V == 8 ? 2 * sizeof(T) : 1];
+
+  // Elements c .. c + V - 1; zeros from n on (with V = 8, n is a multiple of 8
+  // and the address 16-byte aligned).
+  __device__ __forceinline__ void load(const T *p, int c, int n) {
+    if constexpr (V == 8) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        *reinterpret_cast<uint4 *>(w + 4 * i) =
+            c < n ? __ldg(reinterpret_cast<const uint4 *>(p + c) + i) : make_uint4(0, 0, 0, 0);
+    } else {
+      *reinterpret_cast<T *>(w) = c < n ? p[c] : T(0.0f);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (uint32_t &u : w) u = 0;
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    } else {
+      return to_f32(reinterpret_cast<const T *>(w)[i]);
+    }
+  }
+};
 
 // 8 consecutive elements, the pointer 16-byte aligned.
 template <typename T>

@@ -14,10 +14,8 @@
 // each CTA loads its 128 of M and half of the N side and keeps 128 rows of D.
 // Against a CTA's own 128 x 256 tile this moves 32 KB rather than 48 KB from L2
 // for the same products, and L2 to SM traffic is what bounded that kernel (54
-// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of 3
-// stages (128 elements of K of both sides; 6 of 64 cost a wait, a commit and an
-// election twice as often, 560 cycles a 64 where the MMAs take 2 N) full by TMA
-// across items, the even
+// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of 6
+// blocks (64 elements of K of both sides) full by TMA across items, the even
 // CTA's issuing warp issues the pair's MMAs into two accumulator buffers of 256
 // TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
 // odd CTA's issuing warp passes on that its stage has landed.  Tiles that reach
@@ -43,9 +41,17 @@ namespace {
 using namespace tcp;
 
 constexpr int kTM = 256, kTN = 256, kTK = 64;  // tile of a pair; kTK elements are 128 bytes
-constexpr int kStages = 6, kSub = 1;  // a stage holds kSub times kTK
 constexpr uint32_t kABytes = kTM / 2 * 128, kSubBytes = (kTM + kTN) / 2 * 128;  // of a CTA
-constexpr uint32_t kStageBytes = kSub * kSubBytes;
+constexpr int kBlocks = 6;                // of kTK in the ring
+// A stage holds kSub blocks of kTK: two halve the waits and commits, which a
+// decoded token pays one by one (15.2 -> 13.5 us); wgrad's sums over an expert's
+// rows are often shorter than two blocks (279 us with one, 284 with two).
+template <int KIND>
+struct Stage {
+  static constexpr int kSub = KIND == kGroupedWgrad ? 1 : 2;
+  static constexpr int kCount = kBlocks / kSub;
+  static constexpr uint32_t kBytes = kSub * kSubBytes;
+};
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.
@@ -54,8 +60,8 @@ constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of
 struct Maps {
   CUtensorMap p[4], q[4];
 };
-constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
-                         (size_t)kStages * kStageBytes + kEpiWarps * kDrainBytes;
+constexpr size_t kSmem = 1024 + sizeof(Pipe<kBlocks>) + sizeof(SegTable) + 16 +
+                         (size_t)kBlocks * kSubBytes + kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
 
 struct Item {
@@ -128,6 +134,8 @@ template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ Maps maps, const GroupedArgs a) {
   constexpr bool kPMn = KIND != kGroupedFwd, kQMn = KIND == kGroupedWgrad;
+  constexpr int kSub = Stage<KIND>::kSub, kStages = Stage<KIND>::kCount;
+  constexpr uint32_t kStageBytes = Stage<KIND>::kBytes;
   extern __shared__ uint8_t smem_raw[];
   using P = Pipe<kStages>;
   P &pp = *reinterpret_cast<P *>(smem_raw);
