@@ -18,19 +18,98 @@
 // stays in the registers of one CTA (8 consecutive values a thread and step)
 // from its loads to its stores, with two block sums forward (sum y^2, then
 // sum x'^2) and two backward (sum x'^2, <c, x'>, sum y^2 together, then S).
-// The gains' gradients are summed in registers over the rows of a CTA, whose
-// sums a second kernel adds in a fixed order.
+// A row's sums wait for the row, so what is on its way decides the bandwidth:
+// where there are more rows than CTAs, a CTA keeps a ring of rows in shared
+// memory full by bulk copies, up to 4 rows ahead (the backward pass with one
+// row ahead in registers reached 2.9 TB/s).  The gains' gradients are summed in
+// registers over the rows of a CTA, whose sums a second kernel adds in a fixed
+// order.
 #include <algorithm>
 
 #include "../../include/moe_b200.h"
 #include "common.cuh"
 #include "cvt.cuh"
 #include "ops.h"
+#include "tma_ptx.cuh"
 
 namespace moe {
 namespace {
 
-constexpr int kMaxThreads = 256;
+constexpr int kMaxThreads = 256, kBwdThreads = 128;
+constexpr int kMaxRing = 4;  // rows ahead
+
+// Rows on their way into shared memory.  A row is up to four tensors' rows one
+// behind the other; a CTA's rows are r, r + gridDim.x, ...
+struct RowRing {
+  uint8_t *mem;
+  uint64_t *full;
+  int *failed;
+  uint32_t row_bytes;
+  int stages;
+  const uint8_t *src[4];
+  int64_t stride[4];
+  uint32_t bytes[4];
+
+  __device__ __forceinline__ RowRing(uint8_t *m, uint64_t *f, int *fail, int n)
+      : mem(m), full(f), failed(fail), row_bytes(0), stages(n) {}
+  __device__ __forceinline__ void tensor(int i, const void *p, int64_t row_stride, uint32_t n) {
+    src[i] = reinterpret_cast<const uint8_t *>(p);
+    stride[i] = row_stride;
+    bytes[i] = p ? n : 0;
+    row_bytes += bytes[i];
+  }
+  __device__ __forceinline__ uint32_t offset(int i) const {
+    uint32_t o = 0;
+    for (int j = 0; j < i; ++j) o += bytes[j];
+    return o;
+  }
+  __device__ __forceinline__ void issue(int s, int64_t r) {  // one thread
+    tma::mbar_expect_tx(&full[s], row_bytes);
+    uint8_t *dst = mem + (size_t)s * row_bytes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!bytes[i]) continue;
+      tma::load_bulk(dst, src[i] + r * stride[i], &full[s], bytes[i]);
+      dst += bytes[i];
+    }
+  }
+  __device__ __forceinline__ void start(int64_t rows) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < stages; ++s) tma::mbar_init(&full[s], 1);
+      *failed = 0;
+      tma::fence_mbar_init();
+      for (int s = 0; s < stages; ++s)
+        if (blockIdx.x + (int64_t)s * gridDim.x < rows) issue(s, blockIdx.x + (int64_t)s * gridDim.x);
+    }
+    __syncthreads();
+  }
+  // Behind a barrier that follows the reads of stage s: the row that takes its
+  // place, and the stage after it.
+  __device__ __forceinline__ void refill(int &s, uint32_t &use, int64_t r, int64_t rows) {
+    if (threadIdx.x == 0 && r + (int64_t)stages * gridDim.x < rows)
+      issue(s, r + (int64_t)stages * gridDim.x);
+    if (++s == stages) {
+      s = 0;
+      ++use;
+    }
+  }
+  // Copies in flight land before the CTA exits after a failed wait.
+  __device__ __forceinline__ void finish(uint32_t *status) {
+    if (!*(volatile int *)failed) return;
+    if (threadIdx.x == 0) {
+      set_status(status, kStatusTimeout);
+      for (int s = 0; s < stages; ++s)
+        for (uint32_t p = 0; p < 2; ++p) tma::mbar_wait(&full[s], p, nullptr, tma::kWaitCycles / 64);
+    }
+    __syncthreads();
+  }
+  // A row that does not arrive in time is recorded; the threads leave together
+  // behind their next barrier.
+  __device__ __forceinline__ const uint8_t *wait(int s, uint32_t use) {
+    if (!tma::mbar_try(&full[s], use & 1) && !tma::mbar_wait(&full[s], use & 1, failed)) *failed = 1;
+    return mem + (size_t)s * row_bytes;
+  }
+};
 
 // Sums of N values over the block; every thread gets them.  Two alternating
 // halves of `buf`, so that one barrier a call is enough.
@@ -75,14 +154,14 @@ __device__ __forceinline__ void load_gain(Piece<float, V> &w, const float *g, in
 }
 
 template <typename TX, typename TY, int V, int NE>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(BlockNormArgs a) {
+__global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const BlockNormArgs a) {
   __shared__ float buf[8][kMaxThreads / 32];
   int flip = 0;
   const int64_t r = blockIdx.x;
   const int H = a.H;
   const float inv_h = 1.0f / (float)H;
   const bool post = a.y && a.post;
-  // everything a row needs is on its way before the first sum
+  // everything the row needs is on its way before the first sum
   Piece<TX, V> x[NE];
   Piece<TY, V> y[NE];
   Piece<float, V> wq[NE], wp[NE];
@@ -130,105 +209,124 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(BlockNormArgs a
   }
 }
 
-// What the backward pass reads of a row.
-template <typename TX, typename TY, int V>
-struct BwdRow {
-  Piece<TX, V> x, d;
-  Piece<TY, V> c, y;
-  __device__ __forceinline__ void load(const BlockNormArgs &a, int64_t r, int at) {
-    const int H = r < a.rows ? a.H : 0;
-    x.load(reinterpret_cast<const TX *>(a.x) + r * a.ld_res, at, H);
-    if (a.dx_out) d.load(reinterpret_cast<const TX *>(a.dx_out) + r * a.ld_res, at, H);
-    else d.clear();
-    if (a.dh) c.load(reinterpret_cast<const TY *>(a.dh) + r * a.ld_blk, at, H);
-    else c.clear();
-    if (a.y) y.load(reinterpret_cast<const TY *>(a.y) + r * a.ld_blk, at, H);
-    else y.clear();
-  }
-};
-
-template <typename TX, typename TY, int V, int NE>
-__global__ void __launch_bounds__(kMaxThreads) block_norm_bwd_kernel(BlockNormArgs a) {
+// RING: rows through shared memory; else straight into registers.
+template <typename TX, typename TY, int V, int NE, bool RING>
+__global__ void __launch_bounds__(kBwdThreads, RING && V * NE <= 16 ? 4 : 1)
+    block_norm_bwd_kernel(const BlockNormArgs a, int stages) {
   __shared__ float buf[8][kMaxThreads / 32];
+  __shared__ uint64_t full[kMaxRing];
+  __shared__ int failed;
+  extern __shared__ __align__(16) uint8_t ring_mem[];
   int flip = 0;
   const int H = a.H;
   const float inv_h = 1.0f / (float)H;
   const bool post = a.y && a.post;
-  // The next row is loaded before this one's sums where its registers allow.
-  constexpr bool kAhead = V * NE <= 8;
-  float wpre[NE][V] = {}, wpost[NE][V] = {};  // sums of the gains' gradients
+  RowRing ring(ring_mem, full, &failed, stages);
+  if (RING) {
+    ring.tensor(0, a.x, a.ld_res * sizeof(TX), H * sizeof(TX));
+    ring.tensor(1, a.dx_out, a.ld_res * sizeof(TX), H * sizeof(TX));
+    ring.tensor(2, a.dh, a.ld_blk * sizeof(TY), H * sizeof(TY));
+    ring.tensor(3, a.y, a.ld_blk * sizeof(TY), H * sizeof(TY));
+    ring.start(a.rows);
+  }
+  const uint32_t od = ring.offset(1), oc = ring.offset(2), oy = ring.offset(3);
+  // The gains stay in registers where a thread has little of the row.
+  constexpr bool kKeep = V * NE <= 16;
   Piece<float, V> gq[NE], gp[NE];
-  BwdRow<TX, TY, V> next[NE];
+  if (kKeep) {
 #pragma unroll
-  for (int n = 0; n < NE; ++n) {
-    const int at = (n * blockDim.x + threadIdx.x) * V;
-    if (kAhead) {
-      load_gain<V>(gq[n], a.w_pre, at, H);
-      load_gain<V>(gp[n], post ? a.w_post : nullptr, at, H);
-      next[n].load(a, blockIdx.x, at);
+    for (int n = 0; n < NE; ++n) {
+      load_gain<V>(gq[n], a.w_pre, (n * blockDim.x + threadIdx.x) * V, H);
+      load_gain<V>(gp[n], post ? a.w_post : nullptr, (n * blockDim.x + threadIdx.x) * V, H);
     }
   }
+  float wpre[NE][V] = {}, wpost[NE][V] = {};  // sums of the gains' gradients
+  TX *dx_row = reinterpret_cast<TX *>(a.dx) + blockIdx.x * a.ld_res;
+  TY *dy_row = reinterpret_cast<TY *>(a.dy) + blockIdx.x * a.ld_blk;
+  int st = 0;
+  uint32_t use = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    BwdRow<TX, TY, V> row[NE];
-    float s[3] = {0.0f, 0.0f, 0.0f};
+    Piece<TX, V> x[NE], dx[NE];
+    Piece<TY, V> ch[NE], y[NE];
+    const uint8_t *mem = RING ? ring.wait(st, use) : nullptr;
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
       const int at = (n * blockDim.x + threadIdx.x) * V;
-      if (kAhead) {
-        row[n] = next[n];
-        next[n].load(a, r + gridDim.x, at);
+      if constexpr (RING) {
+        x[n].load_shared(mem, at, H);
+        if (a.dx_out) dx[n].load_shared(mem + od, at, H);
+        if (a.dh) ch[n].load_shared(mem + oc, at, H);
+        if (a.y) y[n].load_shared(mem + oy, at, H);
       } else {
-        row[n].load(a, r, at);
-        load_gain<V>(gq[n], a.w_pre, at, H);
+        x[n].load(reinterpret_cast<const TX *>(a.x) + r * a.ld_res, at, H);
+        if (a.dx_out) dx[n].load(reinterpret_cast<const TX *>(a.dx_out) + r * a.ld_res, at, H);
+        if (a.dh) ch[n].load(reinterpret_cast<const TY *>(a.dh) + r * a.ld_blk, at, H);
+        if (a.y) y[n].load(reinterpret_cast<const TY *>(a.y) + r * a.ld_blk, at, H);
       }
+      if (!a.dx_out) dx[n].clear();
+      if (!a.dh) ch[n].clear();
+      if (!a.y) y[n].clear();
+    }
+    if (RING) {
+      __syncthreads();  // the row is in registers
+      if (*(volatile int *)&failed) break;
+      ring.refill(st, use, r, a.rows);
+    }
+    float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < NE; ++n) {
+      if (!kKeep) load_gain<V>(gq[n], a.w_pre, (n * blockDim.x + threadIdx.x) * V, H);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[0] = fmaf(row[n].x[i], row[n].x[i], s[0]);
-        s[1] = fmaf(row[n].c[i] * gq[n][i], row[n].x[i], s[1]);
-        s[2] = fmaf(row[n].y[i], row[n].y[i], s[2]);
+        const float xv = x[n][i], yv = y[n][i];
+        s[0] = fmaf(xv, xv, s[0]);
+        s[1] = fmaf(gq[n][i], ch[n][i] * xv, s[1]);
+        s[2] = fmaf(yv, yv, s[2]);
       }
     }
     block_sums(s, buf, flip);
     const float rq = a.dh ? __frsqrt_rn(s[0] * inv_h + a.eps) : 0.0f;
     const float rp = post ? __frsqrt_rn(s[2] * inv_h + a.eps) : 1.0f;
     const float kx = rq * rq * rq * s[1] * inv_h;
-    const float g = a.y && a.gate ? a.gate[r] : 1.0f;
+    const float grp = (a.y && a.gate ? a.gate[r] : 1.0f) * rp;
     float t[1] = {0.0f}, d[NE][V];
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
       const int at = (n * blockDim.x + threadIdx.x) * V;
-      if (!kAhead) {
+      if (!kKeep) {
         load_gain<V>(gq[n], a.w_pre, at, H);
         load_gain<V>(gp[n], post ? a.w_post : nullptr, at, H);
       }
       float o[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float x = row[n].x[i], c = row[n].c[i];
-        wpre[n][i] = fmaf(c, x * rq, wpre[n][i]);
-        d[n][i] = fmaf(rq, c * gq[n][i], row[n].d[i]) - kx * x;
-        o[i] = a.scale * d[n][i];
-        wpost[n][i] = fmaf(g * d[n][i], row[n].y[i] * rp, wpost[n][i]);
-        d[n][i] *= gp[n][i];
-        t[0] = fmaf(d[n][i], row[n].y[i], t[0]);
+        const float xv = x[n][i], c = ch[n][i];
+        wpre[n][i] = fmaf(rq, c * xv, wpre[n][i]);
+        const float D = fmaf(-kx, xv, fmaf(rq, c * gq[n][i], dx[n][i])), Dy = D * y[n][i];
+        o[i] = a.scale * D;
+        wpost[n][i] = fmaf(grp, Dy, wpost[n][i]);
+        t[0] = fmaf(gp[n][i], Dy, t[0]);
+        d[n][i] = D * gp[n][i];
       }
-      store_v<TX, V>(reinterpret_cast<TX *>(a.dx) + r * a.ld_res, at, H, o);
+      store_v<TX, V>(dx_row, at, H, o);
     }
+    dx_row += (int64_t)gridDim.x * a.ld_res;
     if (!a.y) continue;
     float ky = 0.0f;
     if (post || a.dgate) {
       block_sums(t, buf, flip);
-      if (post) ky = rp * rp * t[0] * inv_h;
+      if (post) ky = -grp * rp * rp * t[0] * inv_h;
       if (a.dgate && threadIdx.x == 0) a.dgate[r] = rp * t[0];
     }
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[n][i] = g * rp * (d[n][i] - ky * row[n].y[i]);
-      store_v<TY, V>(reinterpret_cast<TY *>(a.dy) + r * a.ld_blk,
-                     (n * blockDim.x + threadIdx.x) * V, H, d[n]);
+      for (int i = 0; i < V; ++i) d[n][i] = fmaf(ky, y[n][i], grp * d[n][i]);
+      store_v<TY, V>(dy_row, (n * blockDim.x + threadIdx.x) * V, H, d[n]);
     }
+    dy_row += (int64_t)gridDim.x * a.ld_blk;
   }
+  if (RING) ring.finish(a.status);
   float *part = a.partial + (int64_t)blockIdx.x * 2 * H;
 #pragma unroll
   for (int n = 0; n < NE; ++n)
@@ -265,27 +363,35 @@ __global__ void __launch_bounds__(1024) block_norm_gains_kernel(const float *par
   }
 }
 
+size_t type_bytes(int dt) { return dt == MOE_DT_F32 ? 4 : 2; }
+
+// Four CTAs an SM, whose rings share its 227 KB.
+constexpr int kCtasPerSm = 4;
+constexpr size_t kRingBytes = 56 * 1024;
+
 // Threads of a row: whole warps that cover it once, 256 at most.
-int row_threads(int H, int v) {
+int row_threads(int H, int v, int most) {
   const int need = (H + v - 1) / v;
-  return std::min(kMaxThreads, (need + 31) / 32 * 32);
+  return std::min(most, (need + 31) / 32 * 32);
 }
 
 // Calls f(integral V, integral NE) for a row of H values: V = 8 where every
 // pointer and row stride allows 16-byte accesses and H is a multiple of 8.
 template <typename F>
-cudaError_t by_width(int H, bool vec, F &&f) {
-  const int ne = (H + (vec ? 8 : 1) * kMaxThreads - 1) / ((vec ? 8 : 1) * kMaxThreads);
+cudaError_t by_width(int H, bool vec, int threads, F &&f) {
+  const int v = vec ? 8 : 1, ne = (H + v * threads - 1) / (v * threads);
   if (vec) {
     if (ne <= 1) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
     if (ne <= 2) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
     if (ne <= 4) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
-    return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+    if (ne <= 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+    return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 16>{});
   }
   if (ne <= 4) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
   if (ne <= 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
   if (ne <= 16) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
+  if (ne <= 64) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
+  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 128>{});
 }
 
 template <typename F>
@@ -312,16 +418,17 @@ bool vec_ok(const BlockNormArgs &a) {
 
 int block_norm_backward_ctas(int rows, int H, int sm_count) {
   (void)H;
-  return std::max(1, std::min(rows, sm_count * 3));
+  return std::max(1, std::min(rows, sm_count * kCtasPerSm));
 }
 
 cudaError_t launch_block_norm(const BlockNormArgs &a, cudaStream_t s) {
   if (a.rows <= 0) return cudaSuccess;
-  const bool vec = vec_ok(a);
   return by_types(a.res_dtype, a.dtype, [&](auto tx, auto ty) {
-    return by_width(a.H, vec, [&](auto v, auto ne) {
-      block_norm_kernel<decltype(tx), decltype(ty), v(), ne()>
-          <<<a.rows, row_threads(a.H, v()), 0, s>>>(a);
+    return by_width(a.H, vec_ok(a), kMaxThreads, [&](auto v, auto ne) {
+      if constexpr (v() * ne() > 64) return cudaErrorInvalidValue;  // wider than kMaxNormWidth
+      else
+        block_norm_kernel<decltype(tx), decltype(ty), v(), ne()>
+            <<<a.rows, row_threads(a.H, v(), kMaxThreads), 0, s>>>(a);
       return cudaGetLastError();
     });
   });
@@ -330,10 +437,24 @@ cudaError_t launch_block_norm(const BlockNormArgs &a, cudaStream_t s) {
 cudaError_t launch_block_norm_backward(const BlockNormArgs &a, cudaStream_t s) {
   const int ctas = block_norm_backward_ctas(a.rows, a.H, a.sm_count);
   const bool vec = vec_ok(a);
+  const size_t row = (size_t)a.H * (type_bytes(a.res_dtype) * (a.dx_out ? 2 : 1) +
+                                    type_bytes(a.dtype) * ((a.dh ? 1 : 0) + (a.y ? 1 : 0)));
+  const int stages = vec && a.rows > ctas ? (int)std::min<size_t>(kMaxRing, kRingBytes / row) : 0;
   cudaError_t e = by_types(a.res_dtype, a.dtype, [&](auto tx, auto ty) {
-    return by_width(a.H, vec, [&](auto v, auto ne) {
-      block_norm_bwd_kernel<decltype(tx), decltype(ty), v(), ne()>
-          <<<ctas, row_threads(a.H, v()), 0, s>>>(a);
+    return by_width(a.H, vec, kBwdThreads, [&](auto v, auto ne) {
+      const int threads = row_threads(a.H, v(), kBwdThreads);
+      if constexpr (v() == 8) {
+        if (stages >= 2) {
+          auto *kernel = block_norm_bwd_kernel<decltype(tx), decltype(ty), v(), ne(), true>;
+          static const cudaError_t attr = cudaFuncSetAttribute(
+              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+          if (attr != cudaSuccess) return attr;
+          kernel<<<ctas, threads, stages * row, s>>>(a, stages);
+          return cudaGetLastError();
+        }
+      }
+      block_norm_bwd_kernel<decltype(tx), decltype(ty), v(), ne(), false>
+          <<<ctas, threads, 0, s>>>(a, 0);
       return cudaGetLastError();
     });
   });

@@ -21,6 +21,16 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
   return __float2bfloat16_rn(v);
 }
 
+// Two values rounded into one word, the first in the low half.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 // V = 8 or 1 elements of a row, as they lie in memory: what a thread holds of a
 // row that is still on its way.
 template <typename T, int V>
@@ -38,6 +48,13 @@ struct Piece {
     } else {
       *reinterpret_cast<T *>(w) = c < n ? p[c] : T(0.0f);
     }
+  }
+  // The same from shared memory (V = 8).
+  __device__ __forceinline__ void load_shared(const uint8_t *p, int c, int n) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      *reinterpret_cast<uint4 *>(w + 4 * i) =
+          c < n ? reinterpret_cast<const uint4 *>(p + c * sizeof(T))[i] : make_uint4(0, 0, 0, 0);
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -76,11 +93,8 @@ __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
     reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
-    uint4 u;
-    T *e = reinterpret_cast<T *>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4 *>(p) = u;
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1], T{}), pack2(v[2], v[3], T{}),
+                                               pack2(v[4], v[5], T{}), pack2(v[6], v[7], T{}));
   }
 }
 

@@ -78,6 +78,7 @@ struct BlockNormArgs {
   void *dx, *dy;
   float *dw_pre, *dw_post, *dgate, *partial;
   int sm_count;
+  uint32_t *status;
 };
 cudaError_t launch_block_norm(const BlockNormArgs &a, cudaStream_t s);
 cudaError_t launch_block_norm_backward(const BlockNormArgs &a, cudaStream_t s);

@@ -241,6 +241,7 @@ moe_status check_norm(moe_handle *h, const moe_block_norm_desc *d, BlockNormArgs
   a.scale = d->residual_scale;
   a.eps = d->eps;
   a.sm_count = h->sm_count;
+  a.status = h->status;
   return MOE_OK;
 }
 

@@ -182,15 +182,6 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) {
 // are parted on the way out.
 constexpr int kDrainBytes = 1024;  // of shared memory, for each draining warp
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
-
 // 8 (4 of fp32) elements of a row, of which the first `left` are inside it.
 template <typename T>
 __device__ __forceinline__ void store_piece(T *p, uint4 v, int left) {

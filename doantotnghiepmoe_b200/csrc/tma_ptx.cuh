@@ -79,5 +79,16 @@ __device__ __forceinline__ void load_3d(void *dst, const void *map, uint64_t *ba
       : "memory");
 }
 
+// `bytes` (a multiple of 16) from global memory into this CTA's shared memory,
+// both 16-byte aligned; counted on bar in bytes.
+__device__ __forceinline__ void load_bulk(void *dst, const void *src, uint64_t *bar,
+                                          uint32_t bytes) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          su32(dst)),
+      "l"(src), "r"(bytes), "r"(su32(bar))
+      : "memory");
+}
+
 }  // namespace tma
 }  // namespace moe
