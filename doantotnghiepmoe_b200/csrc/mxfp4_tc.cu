@@ -38,11 +38,21 @@ constexpr int kScaleBytes = 6 * kGroup;  // of a stage: 2 groups of w, 2 x 2 of 
 constexpr int kSetCols = 24;             // TMEM columns of a stage's scales
 constexpr uint32_t kTmemCols = 512;
 static_assert(2 * kTN + kStages * kSetCols <= (int)kTmemCols, "TMEM");
+// A warp comes to a stage every time round or less often, never two rounds late:
+// the parity of a wait names one round only.
 constexpr int kScaleWarps = 4;
+static_assert(kScaleWarps <= kStages, "scale warps");
 constexpr int kMxThreads = kThreads + 32 * kScaleWarps;
 constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
                          (size_t)kStages * (kStageBytes + kScaleBytes) + kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
+
+// A lane's scale words of a step (256 elements of K): words 2 kb and 2 kb + 1 of
+// rows 32 i + lane of w (i < 4) and of x (i - 4).
+struct Scales {
+  uint2 u[10];
+  bool wide;  // more than 128 rows of x
+};
 
 struct Maps {
   CUtensorMap w, x[3];  // x in boxes of 64, 32 and 16 rows
@@ -163,35 +173,66 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     const int words = mxfp4_scale_stride(a.k) / 4;
     const uint32_t *xs = reinterpret_cast<const uint32_t *>(a.xs);
     const uint32_t *ws = reinterpret_cast<const uint32_t *>(a.ws);
-    int w = blockIdx.x;
-    int kb = warp - 3;  // this warp's steps: every kScaleWarps-th
-    for (int q = warp - 3;; q += kScaleWarps, kb += kScaleWarps) {
+    // both words of a step in one load, where that is aligned
+    const bool even = words % 2 == 0 && (((uintptr_t)xs | (uintptr_t)ws) & 7) == 0;
+    // This warp's steps are every kScaleWarps-th; the next one's words are loaded
+    // before this one's are stored.
+    int w = blockIdx.x, kb = warp - 3, it_w = -1;
+    Item it{};
+    Scales cur, next;
+    const auto advance = [&] {  // to the item that holds step kb; false behind the last
       for (; kb >= nk && w < total; kb -= nk) w += gridDim.x;
-      if (w >= total) break;
-      const Item it = item(w);
-      // v[g]: the words of rows l, l + 32, l + 64, l + 96 of w, then of x twice
-      uint32_t v[2][12];
-#pragma unroll
-      for (int i = 0; i < 12; ++i) {
-        const int r = i % 4 * 32 + (i < 8 ? 0 : 128) + lane;
-        const bool in = i < 4 ? it.m0 + r < a.n : r < it.nc;
-        const uint32_t *row = i < 4 ? ws + ((int64_t)it.e * a.n + it.m0 + r) * words
-                                    : xs + ((int64_t)it.c0 + r) * words;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          v[g][i] = in && 2 * kb + g < words ? __ldg(row + 2 * kb + g) : 0u;
+      if (w >= total) return false;
+      if (w != it_w) {
+        it = item(w);
+        it_w = w;
       }
+      return true;
+    };
+    const auto load = [&](Scales &v) {
+      const uint32_t *wrow = ws + ((int64_t)it.e * a.n + it.m0) * words + 2 * kb + lane * words;
+      const uint32_t *xrow = xs + (int64_t)it.c0 * words + 2 * kb + lane * words;
+      const bool two = 2 * kb + 1 < words;
+#pragma unroll
+      for (int i = 0; i < 10; ++i) {
+        const int r0 = (i < 4 ? i : i - 4) * 32, left = (i < 4 ? a.n - it.m0 : it.nc) - r0;
+        const uint32_t *p = (i < 4 ? wrow : xrow) + r0 * words;
+        uint2 u = make_uint2(0u, 0u);
+        if (left > 0) {  // warp-uniform
+          if (lane < left) {
+            if (two && even) {
+              u = __ldg(reinterpret_cast<const uint2 *>(p));
+            } else {
+              u.x = __ldg(p);
+              if (two) u.y = __ldg(p + 1);
+            }
+          }
+        }
+        v.u[i] = u;
+      }
+      v.wide = it.nc > 128;
+    };
+    bool more = advance();
+    if (more) load(cur);
+    for (int q = warp - 3; more; q += kScaleWarps) {
+      kb += kScaleWarps;
+      more = advance();
+      if (more) load(next);
       const int s = q % kStages, use = q / kStages;
       if (use > 0 && !pp.wait_warp(&pp.empty[s], (use - 1) & 1)) break;
       uint4 *dst = reinterpret_cast<uint4 *>(scales + s * kScaleBytes) + lane;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        dst[g * 32] = make_uint4(v[g][0], v[g][1], v[g][2], v[g][3]);
-        dst[(2 + 2 * g) * 32] = make_uint4(v[g][4], v[g][5], v[g][6], v[g][7]);
-        dst[(3 + 2 * g) * 32] = make_uint4(v[g][8], v[g][9], v[g][10], v[g][11]);
+      const uint2(&u)[10] = cur.u;
+      dst[0] = make_uint4(u[0].x, u[1].x, u[2].x, u[3].x);
+      dst[32] = make_uint4(u[0].y, u[1].y, u[2].y, u[3].y);
+      dst[64] = make_uint4(u[4].x, u[5].x, u[6].x, u[7].x);
+      dst[128] = make_uint4(u[4].y, u[5].y, u[6].y, u[7].y);
+      if (cur.wide) {
+        dst[96] = make_uint4(u[8].x, u[9].x, 0u, 0u);
+        dst[160] = make_uint4(u[8].y, u[9].y, 0u, 0u);
       }
       tma::fence_proxy_async_smem();  // before the tensor cores' proxy reads them
       tma::mbar_arrive(&pp.full[s]);
+      cur = next;
     }
   } else {
     const int ew = warp - 3 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;

@@ -201,6 +201,11 @@ class MoeLayerEngine:
         import torch
         return torch.device("cuda", self.device)
 
+    @cached_property
+    def _bytes(self):
+        import torch
+        return torch.empty(0, dtype=torch.uint8, device=self._dev)
+
     def _bad(self, name, t, want):
         raise MoeError(MOE_ERR_INVALID, f"{name}: {want} on cuda:{self.device} wanted, got "
                        f"{t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}")
@@ -268,10 +273,8 @@ class MoeLayerEngine:
 
     def mxfp4_empty(self, rows: int, k: int):
         """Uninitialised (codes, scales) of `rows` MXFP4 rows of k values."""
-        import torch
         lc, ls = mxfp4_strides(k)
-        return (torch.empty((rows, lc), dtype=torch.uint8, device=self._dev),
-                torch.empty((rows, ls), dtype=torch.uint8, device=self._dev))
+        return self._bytes.new_empty(rows, lc), self._bytes.new_empty(rows, ls)
 
     def _mxfp4(self, name, codes, scales, rows, k):
         import torch
@@ -376,11 +379,11 @@ class MoeLayerEngine:
         need = L.moe_block_norm_backward_workspace(self._h, d.rows, d.hidden)
         s = _op_stream(stream) or L.moe_get_stream(self._h)
         if s == _op_stream(torch.cuda.current_stream(self._dev)):
-            ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+            ws = self._bytes.new_empty(need)
         else:  # from the pool of the stream that uses it: its reuse is ordered there
             with torch.cuda.stream(torch.cuda.default_stream(self._dev) if s == 1 else
                                    torch.cuda.ExternalStream(s, device=self._dev)):
-                ws = torch.empty(need, dtype=torch.uint8, device=self._dev)
+                ws = self._bytes.new_empty(need)
         self._check(L.moe_block_norm_backward(self._h, d, _ptr(dx_out), _ptr(dh), x_out.data_ptr(),
                                               _ptr(y), _ptr(w_post), _ptr(gate), _ptr(w_pre),
                                               dx.data_ptr(), _ptr(dy), _ptr(dw_post), _ptr(dgate),
