@@ -48,6 +48,12 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // of 16-bit halves
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Eight values of a row as they lie in memory; for fp32 as their bits.
 template <typename T>
 struct Raw8 {
@@ -66,21 +72,32 @@ struct Raw8 {
     }
   }
   __device__ __forceinline__ float value(int i) const {
-    return to_f32(reinterpret_cast<const T *>(w)[i]);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+      return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return to_f32(reinterpret_cast<const T *>(w)[i]);
   }
-  // The fp32 bits of the largest magnitude; any NaN counts above infinity.
-  __device__ __forceinline__ uint32_t top() const {
+  // The exponent field of the largest magnitude of the four lanes' 32 values in
+  // fp32 (any NaN counts above infinity, as an integer): on pairs of 16-bit
+  // magnitudes where the values are that.
+  __device__ __forceinline__ uint32_t top_exponent() const {
     if constexpr (sizeof(T) == 2) {
-      const uint32_t m =
-          __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
-                   __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-      const unsigned short h = (unsigned short)max(m & 0xffffu, m >> 16);
-      return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+      uint32_t m = max2(max2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                        max2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+      m = max2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      m = max(m & 0xffffu, m >> 16);
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        return m >> 7;
+      } else {
+        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))) >> 23;
+      }
     } else {
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
-      return m;
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      return m >> 23;
     }
   }
 };
@@ -114,6 +131,7 @@ __global__ void __launch_bounds__(kQThreads) mxfp4_quantize_kernel(Mxfp4Quant a,
       }
     }
     const T *row = reinterpret_cast<const T *>(a.x) + src * a.ld_x;
+    uint8_t *codes = a.codes + r * ldc, *scales = a.scales + r * lds;
     for (int s0 = sw.part; s0 < spans; s0 += kFlight * sw.parts) {
       Raw8<T> x[kFlight];
 #pragma unroll
@@ -123,40 +141,42 @@ __global__ void __launch_bounds__(kQThreads) mxfp4_quantize_kernel(Mxfp4Quant a,
       for (int f = 0; f < kFlight; ++f) {
         const int c = (s0 + f * sw.parts) * kSpan + sw.lane * 8, blk = c / 32;
         if (s0 + f * sw.parts >= spans) break;  // warp-uniform
-        uint32_t m = x[f].top();
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t ex = m >> 23;  // floor(log2 max) + 127 (0 for subnormal numbers)
-        const uint32_t sb = ex == 255u ? 255u : (ex > 2u ? ex - 2u : 0u);
-        const float inv = __uint_as_float((254u - min(sb, 252u)) << 23);  // 2^(127 - sb), normal
+        const uint32_t ex = x[f].top_exponent();  // floor(log2 max) + 127, 0 if subnormal
+        const uint32_t sb = max(ex, 2u) - 2u;
+        const float inv = __uint_as_float((254u - sb) << 23);  // 2^(127 - sb), a normal number
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = x[f].value(i) * inv;
-        const uint32_t q = ex == 255u ? 0u : e2m1x8(v);
-        if (blk < nb) *reinterpret_cast<uint32_t *>(a.codes + r * ldc + c / 2) = q;
-        // a warp's span has 8 scales; two lanes store 4 of them each
-        uint32_t word = blk < nb ? sb << (sw.lane / 4 % 4 * 8) : 0u;
-        word |= __shfl_xor_sync(0xffffffffu, word, 4);
-        word |= __shfl_xor_sync(0xffffffffu, word, 8);
-        if (sw.lane % 16 == 0 && blk < lds)
-          *reinterpret_cast<uint32_t *>(a.scales + r * lds + blk) = word;
+        const uint32_t q = e2m1x8(v);
+        const bool bad = ex == 255u;
+        if (blk < nb) *reinterpret_cast<uint32_t *>(codes + c / 2) = bad ? 0u : q;
+        if ((sw.lane & 3) == 0 && blk < lds)
+          scales[blk] = (uint8_t)(blk >= nb ? 0u : bad ? 255u : sb);
       }
     }
   }
 }
 
-// The bf16 of the eight codes in q, codes 2i and 2i + 1 in word i: the bytes of
-// 0 0.5 1 1.5 2 3 4 6 are looked up by the codes' low three bits.
+// __byte_perm with all four bits of each selector.
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
+  return r;
+}
+
+// The bf16 of the eight codes in q, codes 2i and 2i + 1 in word i.  The high and
+// low bytes of 0 0.5 1 1.5 2 3 4 6 are looked up by the codes' low three bits;
+// with the fourth bit set a lookup repeats the byte's top bit instead, which
+// makes 0xff of 0x80 and so the sign.
 __device__ __forceinline__ void e2m1x8_bf16(uint32_t q, uint32_t (&w)[4]) {
-  const uint32_t sel = q & 0x77777777u;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t s = sel >> (16 * h);
-    const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, s);
-    const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, s);
-    const uint32_t sg = q >> (16 * h);
-    w[2 * h] = __byte_perm(lo, hi, 0x5140) | (sg & 8u) << 12 | (sg & 0x80u) << 24;
-    w[2 * h + 1] = __byte_perm(lo, hi, 0x7362) | (sg & 0x800u) << 4 | (sg & 0x8000u) << 16;
+    const uint32_t t = q >> (16 * h), sel = t & 0x7777u;
+    const uint32_t sg = prmt(0x80808080u, 0x80808080u, t);
+    const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, sel) | (sg << 7 & 0x80808080u);
+    const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, sel);
+    w[2 * h] = __byte_perm(lo, hi, 0x5140);
+    w[2 * h + 1] = __byte_perm(lo, hi, 0x7362);
   }
 }
 
