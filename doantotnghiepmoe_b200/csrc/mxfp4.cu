@@ -15,11 +15,12 @@
 // Both directions move each byte once and are bound by HBM, with the issue slots
 // close behind, so 16-bit values stay packed: the maximum of a block is taken
 // on pairs of magnitudes, and codes become bf16 by byte lookups (prmt) and one
-// packed multiplication by the scale.  A warp takes 256 values of a row at a
-// time (8 a lane, one 16-byte load of 16-bit values), four such spans in
-// flight: a block is 4 lanes, its maximum two shuffles, and a lane stores its 8
-// codes as one word, so a warp's store is 128 contiguous bytes.  Rows go to
-// warps, or their parts to several (a power of two) where rows are few.
+// packed multiplication by the scale.  A warp quantises 512 values of a row at a
+// time, two such spans in flight: a lane has half a block (8 values a lane took 93
+// instructions for them), so that its maximum is one shuffle, and stores 16
+// codes.  It dequantises 256 at a time, four in flight: 8 codes a lane, whose
+// bf16 values are one 16-byte store.  Rows go to warps, or their parts to several
+// (a power of two) where rows are few.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,8 +32,9 @@
 namespace moe {
 namespace {
 
-constexpr int kQThreads = 256, kSpan = 256;  // values of a warp's step
-constexpr int kFlight = 4;                   // spans whose loads are issued together
+constexpr int kQThreads = 256;
+// Values of a warp's step, and steps whose loads are issued together.
+constexpr int kQuantSpan = 512, kQuantFlight = 2, kSpan = 256, kFlight = 4;
 
 // Codes of eight values already divided by the scale, value i in nibble i.
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
@@ -54,21 +56,21 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // of 16-bit
   return r;
 }
 
-// Eight values of a row as they lie in memory; for fp32 as their bits.
+// Sixteen values of a row, half a block, as they lie in memory.
 template <typename T>
-struct Raw8 {
-  uint32_t w[2 * sizeof(T)];
+struct Half {
+  uint32_t w[4 * sizeof(T)];
 
   template <bool VEC>
   __device__ __forceinline__ void load(const T *row, int c, int k) {
-    if (VEC && c + 8 <= k) {
+    if (VEC && c + 16 <= k) {
       const uint4 *p = reinterpret_cast<const uint4 *>(row + c);
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) *reinterpret_cast<uint4 *>(w + 4 * i) = __ldg(p + i);
+      for (int i = 0; i < (int)sizeof(T); ++i) *reinterpret_cast<uint4 *>(w + 4 * i) = __ldg(p + i);
     } else {
       T *e = reinterpret_cast<T *>(w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = c + i < k ? row[c + i] : T(0.0f);
+      for (int i = 0; i < 16; ++i) e[i] = c + i < k ? row[c + i] : T(0.0f);
     }
   }
   __device__ __forceinline__ float value(int i) const {
@@ -76,15 +78,15 @@ struct Raw8 {
       return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     else return to_f32(reinterpret_cast<const T *>(w)[i]);
   }
-  // The exponent field of the largest magnitude of the four lanes' 32 values in
+  // The exponent field of the largest magnitude of the two lanes' 32 values in
   // fp32 (any NaN counts above infinity, as an integer): on pairs of 16-bit
   // magnitudes where the values are that.
   __device__ __forceinline__ uint32_t top_exponent() const {
     if constexpr (sizeof(T) == 2) {
-      uint32_t m = max2(max2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
-                        max2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+      uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m = max2(m, w[i] & 0x7fff7fffu);
       m = max2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max2(m, __shfl_xor_sync(0xffffffffu, m, 2));
       m = max(m & 0xffffu, m >> 16);
       if constexpr (std::is_same_v<T, __nv_bfloat16>) {
         return m >> 7;
@@ -94,10 +96,8 @@ struct Raw8 {
     } else {
       uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      return m >> 23;
+      for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+      return max(m, __shfl_xor_sync(0xffffffffu, m, 1)) >> 23;
     }
   }
 };
@@ -119,7 +119,7 @@ struct SpanWalk {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQThreads) mxfp4_quantize_kernel(Mxfp4Quant a, int shift) {
   const SpanWalk sw(shift);
-  const int spans = (a.k + kSpan - 1) / kSpan, nb = (a.k + 31) / 32;
+  const int spans = (a.k + kQuantSpan - 1) / kQuantSpan, nb = (a.k + 31) / 32;
   const int ldc = mxfp4_code_stride(a.k), lds = mxfp4_scale_stride(a.k);
   for (long long r = sw.row; r < a.rows; r += sw.step) {
     long long src = r;
@@ -132,25 +132,26 @@ __global__ void __launch_bounds__(kQThreads) mxfp4_quantize_kernel(Mxfp4Quant a,
     }
     const T *row = reinterpret_cast<const T *>(a.x) + src * a.ld_x;
     uint8_t *codes = a.codes + r * ldc, *scales = a.scales + r * lds;
-    for (int s0 = sw.part; s0 < spans; s0 += kFlight * sw.parts) {
-      Raw8<T> x[kFlight];
+    for (int s0 = sw.part; s0 < spans; s0 += kQuantFlight * sw.parts) {
+      Half<T> x[kQuantFlight];
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f)
-        x[f].template load<VEC>(row, (s0 + f * sw.parts) * kSpan + sw.lane * 8, src < 0 ? 0 : a.k);
+      for (int f = 0; f < kQuantFlight; ++f)
+        x[f].template load<VEC>(row, (s0 + f * sw.parts) * kQuantSpan + sw.lane * 16,
+                                src < 0 ? 0 : a.k);
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
-        const int c = (s0 + f * sw.parts) * kSpan + sw.lane * 8, blk = c / 32;
+      for (int f = 0; f < kQuantFlight; ++f) {
+        const int c = (s0 + f * sw.parts) * kQuantSpan + sw.lane * 16, blk = c / 32;
         if (s0 + f * sw.parts >= spans) break;  // warp-uniform
         const uint32_t ex = x[f].top_exponent();  // floor(log2 max) + 127, 0 if subnormal
         const uint32_t sb = max(ex, 2u) - 2u;
         const float inv = __uint_as_float((254u - sb) << 23);  // 2^(127 - sb), a normal number
-        float v[8];
+        float v[2][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = x[f].value(i) * inv;
-        const uint32_t q = e2m1x8(v);
+        for (int i = 0; i < 16; ++i) v[i / 8][i % 8] = x[f].value(i) * inv;
         const bool bad = ex == 255u;
-        if (blk < nb) *reinterpret_cast<uint32_t *>(codes + c / 2) = bad ? 0u : q;
-        if ((sw.lane & 3) == 0 && blk < lds)
+        const uint2 q = bad ? make_uint2(0u, 0u) : make_uint2(e2m1x8(v[0]), e2m1x8(v[1]));
+        if (blk < nb) *reinterpret_cast<uint2 *>(codes + c / 2) = q;
+        if ((sw.lane & 1) == 0 && blk < lds)
           scales[blk] = (uint8_t)(blk >= nb ? 0u : bad ? 255u : sb);
       }
     }
@@ -241,9 +242,9 @@ __global__ void __launch_bounds__(kQThreads) mxfp4_dequantize_kernel(Mxfp4Dequan
 
 // Warps of a row, as a shift: 1, or a power of two up to its spans while the
 // rows alone would leave the GPU's warps idle; and the grid.
-int row_split(int rows, int k, int sm_count, int *grid) {
+int row_split(int rows, int k, int span, int sm_count, int *grid) {
   const long long warps = (long long)sm_count * 8 * (kQThreads / 32);
-  const int spans = (k + kSpan - 1) / kSpan;
+  const int spans = (k + span - 1) / span;
   int shift = 0;
   while ((2 << shift) <= spans && ((long long)rows << (shift + 1)) <= warps) ++shift;
   const long long blocks = (((long long)rows << shift) + kQThreads / 32 - 1) / (kQThreads / 32);
@@ -255,7 +256,7 @@ template <typename T>
 cudaError_t quantize_t(const Mxfp4Quant &a, cudaStream_t s) {
   const bool vec = ((uintptr_t)a.x & 15) == 0 && (a.ld_x * sizeof(T)) % 16 == 0;
   int grid;
-  const int shift = row_split(a.rows, a.k, a.sm_count, &grid);
+  const int shift = row_split(a.rows, a.k, kQuantSpan, a.sm_count, &grid);
   if (vec) mxfp4_quantize_kernel<T, true><<<grid, kQThreads, 0, s>>>(a, shift);
   else mxfp4_quantize_kernel<T, false><<<grid, kQThreads, 0, s>>>(a, shift);
   return cudaGetLastError();
@@ -265,7 +266,7 @@ template <typename T>
 cudaError_t dequantize_t(const Mxfp4Dequant &a, cudaStream_t s) {
   const bool vec = ((uintptr_t)a.out & 15) == 0 && (a.ld_out * sizeof(T)) % 16 == 0;
   int grid;
-  const int shift = row_split(a.rows, a.k, a.sm_count, &grid);
+  const int shift = row_split(a.rows, a.k, kSpan, a.sm_count, &grid);
   if (vec) mxfp4_dequantize_kernel<T, true><<<grid, kQThreads, 0, s>>>(a, shift);
   else mxfp4_dequantize_kernel<T, false><<<grid, kQThreads, 0, s>>>(a, shift);
   return cudaGetLastError();
