@@ -14,8 +14,9 @@
 // each CTA loads its 128 of M and half of the N side and keeps 128 rows of D.
 // Against a CTA's own 128 x 256 tile this moves 32 KB rather than 48 KB from L2
 // for the same products, and L2 to SM traffic is what bounded that kernel (54
-// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of 6
-// blocks (64 elements of K of both sides) full by TMA across items, the even
+// bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of
+// stages full by TMA across items (6 blocks of 64 elements of K of both sides, or
+// more of smaller tiles), the even
 // CTA's issuing warp issues the pair's MMAs into two accumulator buffers of 256
 // TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
 // odd CTA's issuing warp passes on that its stage has landed.  Tiles that reach
@@ -41,17 +42,14 @@ namespace {
 using namespace tcp;
 
 constexpr int kTM = 256, kTN = 256, kTK = 64;  // tile of a pair; kTK elements are 128 bytes
-constexpr uint32_t kABytes = kTM / 2 * 128, kSubBytes = (kTM + kTN) / 2 * 128;  // of a CTA
-constexpr int kBlocks = 6;                // of kTK in the ring
+constexpr uint32_t kABytes = kTM / 2 * 128;  // of a CTA and a block of kTK
+constexpr uint32_t kRingBytes = 6 * (kTM + kTN) / 2 * 128;
 // A stage holds kSub blocks of kTK: two halve the waits and commits, which a
 // decoded token pays one by one (15.2 -> 13.5 us); wgrad's sums over an expert's
 // rows are often shorter than two blocks (279 us with one, 284 with two).
 template <int KIND>
-struct Stage {
-  static constexpr int kSub = KIND == kGroupedWgrad ? 1 : 2;
-  static constexpr int kCount = kBlocks / kSub;
-  static constexpr uint32_t kBytes = kSub * kSubBytes;
-};
+constexpr int kSubOf = KIND == kGroupedWgrad ? 1 : 2;
+constexpr int kMaxStages = 10;
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.
@@ -60,8 +58,8 @@ constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of
 struct Maps {
   CUtensorMap p[4], q[4];
 };
-constexpr size_t kSmem = 1024 + sizeof(Pipe<kBlocks>) + sizeof(SegTable) + 16 +
-                         (size_t)kBlocks * kSubBytes + kEpiWarps * kDrainBytes;
+constexpr size_t kSmem = 1024 + sizeof(Pipe<kMaxStages>) + sizeof(SegTable) + 16 + kRingBytes +
+                         kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
 
 struct Item {
@@ -134,10 +132,9 @@ template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ Maps maps, const GroupedArgs a) {
   constexpr bool kPMn = KIND != kGroupedFwd, kQMn = KIND == kGroupedWgrad;
-  constexpr int kSub = Stage<KIND>::kSub, kStages = Stage<KIND>::kCount;
-  constexpr uint32_t kStageBytes = Stage<KIND>::kBytes;
+  constexpr int kSub = kSubOf<KIND>;
   extern __shared__ uint8_t smem_raw[];
-  using P = Pipe<kStages>;
+  using P = Pipe<kMaxStages>;
   P &pp = *reinterpret_cast<P *>(smem_raw);
   SegTable &seg = *reinterpret_cast<SegTable *>(smem_raw + sizeof(P));
   uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
@@ -154,9 +151,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();
   fence_after_sync();
   const Work<KIND> work(a, seg);
+  // The largest tile's N side decides the stages' size and with it how many fit:
+  // with the few rows of a decode batch they hold the weights alone, and more of
+  // them are on their way.
+  const int half_most = (min(kQMn ? a.n : seg.most, kTN) + 31) / 32 * 16;
+  const uint32_t sub_bytes =
+      kABytes + (kQMn ? (uint32_t)(half_most + 63) / 64 * kMnBox : half_most * 128u);
+  const uint32_t stage_bytes = kSub * sub_bytes;
+  const int stages = min(kMaxStages, (int)(kRingBytes / stage_bytes));
 
   if (warp == 0 || warp == 2) {
-    Ring<kStages> ring;
+    Ring ring(stages);
     bool ok = true;
     for (int w = pair; w < work.total && ok; w += pairs) {
       const Item it = work.item(w);
@@ -166,14 +171,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ok = ring.use == 0 || pp.wait_warp(&pp.empty[ring.s], (ring.use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t *st = tiles + ring.s * kStageBytes;
+          uint8_t *st = tiles + ring.s * stage_bytes;
           uint64_t *bar = &pp.full[ring.s];
           const int left = it.len - k0;  // of the summed axis
           if (warp == 0)
             tma::mbar_expect_tx(
                 bar, kQMn ? (2 + boxes) * 128u * min(kSub * kTK, (left + 15) & ~15)
                           : (kABytes + half * 128u) * (left > kTK ? kSub : 1));
-          for (int sub = 0; sub < kSub; ++sub, st += kSubBytes) {
+          for (int sub = 0; sub < kSub; ++sub, st += sub_bytes) {
             if (sub * kTK >= left) break;
             const int k = k0 + sub * kTK;
             if (warp == 0) {
@@ -213,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr uint64_t kPStep = (kPMn ? 2048 : 32) >> 4, kQStep = (kQMn ? 2048 : 32) >> 4;
     const uint64_t pd0 = sw128_desc(su32(tiles), kPMn ? kMnBox : 16, 1024);
     const uint64_t qd0 = sw128_desc(su32(tiles) + kABytes, kQMn ? kMnBox : 16, 1024);
-    Ring<kStages> ring;
+    Ring ring(stages);
     int j = 0;
     for (int w = pair; w < work.total; w += pairs) {
       const Item it = work.item(w);
@@ -232,12 +237,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (rank != 0) {
           if (elect_one()) arrive_at(&pp.full[ring.s], 0);
         } else if (elect_one()) {
-          const uint64_t at = (uint64_t)(ring.s * (kStageBytes >> 4));
+          const uint64_t at = (uint64_t)(ring.s * (stage_bytes >> 4));
           const int left = it.len - k0;
           if (left >= kSub * kTK || (!kQMn && left > kTK)) {
 #pragma unroll
             for (int k = 0; k < kSub * kTK / 16; ++k) {
-              const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (kSubBytes >> 4);
+              const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (sub_bytes >> 4);
               mma_f16_pair(d, pd0 + sub + k % (kTK / 16) * kPStep,
                            qd0 + sub + k % (kTK / 16) * kQStep, idesc, (k0 > 0 || k > 0) ? 1u : 0u);
             }
@@ -246,7 +251,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // rows there are, in steps of 16
             const int steps = kQMn ? (left + 15) / 16 : kTK / 16;
             for (int k = 0; k < steps; ++k) {
-              const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (kSubBytes >> 4);
+              const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (sub_bytes >> 4);
               mma_f16_pair(d, pd0 + sub + k % (kTK / 16) * kPStep,
                            qd0 + sub + k % (kTK / 16) * kQStep, idesc, (k0 > 0 || k > 0) ? 1u : 0u);
             }
@@ -265,8 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma::mbar_wait(&pp.done, 0, nullptr);
   } else {
     const int quarter = warp & 3, grp = (warp - 3) >> 2;
-    uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kStages * kStageBytes +
-                                                   (warp - 3) * kDrainBytes);
+    uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kRingBytes + (warp - 3) * kDrainBytes);
     const int M = KIND == kGroupedFwd ? a.n : a.k;
     const int64_t ld = KIND == kGroupedFwd ? a.ld_out : KIND == kGroupedDgrad ? a.ld_x : a.ld_w;
     int j = 0;

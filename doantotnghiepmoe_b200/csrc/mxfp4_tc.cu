@@ -31,20 +31,20 @@ namespace {
 using namespace tcp;
 
 constexpr int kTM = 128, kTN = 192;
-constexpr int kStages = 4;
-constexpr uint32_t kABytes = kTM * 128, kBBytes = kTN * 128, kStageBytes = kABytes + kBBytes;
+constexpr uint32_t kABytes = kTM * 128;
+constexpr int kMaxStages = 8;
 constexpr int kGroup = 512;            // scale bytes of 128 rows and 4 blocks
 constexpr int kScaleBytes = 6 * kGroup;  // of a stage: 2 groups of w, 2 x 2 of x
 constexpr int kSetCols = 24;             // TMEM columns of a stage's scales
 constexpr uint32_t kTmemCols = 512;
-static_assert(2 * kTN + kStages * kSetCols <= (int)kTmemCols, "TMEM");
 // A warp comes to a stage every time round or less often, never two rounds late:
 // the parity of a wait names one round only.
 constexpr int kScaleWarps = 4;
-static_assert(kScaleWarps <= kStages, "scale warps");
+static_assert(kScaleWarps <= 4, "the fewest stages of a ring");
 constexpr int kMxThreads = kThreads + 32 * kScaleWarps;
-constexpr size_t kSmem = 1024 + sizeof(Pipe<kStages>) + sizeof(SegTable) + 16 +
-                         (size_t)kStages * (kStageBytes + kScaleBytes) + kEpiWarps * kDrainBytes;
+constexpr uint32_t kRingBytes = 4 * (kABytes + kTN * 128 + kScaleBytes) + 32 * 1024;
+constexpr size_t kSmem = 1024 + sizeof(Pipe<kMaxStages>) + sizeof(SegTable) + 16 + kRingBytes +
+                         kEpiWarps * kDrainBytes;
 static_assert(kSmem <= 232448, "shared memory");
 
 // A lane's scale words of a step (256 elements of K): words 2 kb and 2 kb + 1 of
@@ -61,11 +61,10 @@ struct Maps {
 __global__ void __launch_bounds__(kMxThreads, 1)
     mxfp4_tc_kernel(const __grid_constant__ Maps maps, const Mxfp4Args a) {
   extern __shared__ uint8_t smem_raw[];
-  using P = Pipe<kStages>;
+  using P = Pipe<kMaxStages>;
   P &pp = *reinterpret_cast<P *>(smem_raw);
   SegTable &seg = *reinterpret_cast<SegTable *>(smem_raw + sizeof(P));
   uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
-  uint8_t *scales = tiles + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) pp.init(1 + 32);  // a copying warp (for both), a scale warp's lanes
   if (warp == 1) tmem_alloc(&pp.tmem_base, kTmemCols);
@@ -74,6 +73,15 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   __syncthreads();
   fence_after_sync();
 
+  // The largest tile decides the stages' size and how many fit, and the columns of
+  // an accumulator buffer: 4 stages with 192 rows of x, 8 with the few rows of a
+  // decode batch, whose stages hold the weights and little else.
+  const int most = (seg.most + 15) & ~15;
+  const uint32_t stage_bytes = kABytes + ((uint32_t)most * 128u + 1023u & ~1023u);
+  const int acc_cols = (most + 31) & ~31;
+  const int stages = min(min(kMaxStages, (int)(kRingBytes / (stage_bytes + kScaleBytes))),
+                         ((int)kTmemCols - 2 * acc_cols) / kSetCols);
+  uint8_t *scales = tiles + stages * stage_bytes;
   const int nM = (a.n + kTM - 1) / kTM, nk = (a.k + 255) / 256;
   const int total = seg.total * nM;
   struct Item {
@@ -92,7 +100,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   };
 
   if (warp == 0 || warp == 2) {
-    Ring<kStages> ring;
+    Ring ring(stages);
     bool ok = true;
     for (int w = blockIdx.x; w < total && ok; w += gridDim.x) {
       const Item it = item(w);
@@ -102,7 +110,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         ok = ring.use == 0 || pp.wait_warp(&pp.empty[s], (ring.use - 1) & 1);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t *st = tiles + s * kStageBytes;
+          uint8_t *st = tiles + s * stage_bytes;
           uint64_t *bar = &pp.full[s];
           if (warp == 0) {
             tma::mbar_expect_tx(bar, kABytes + rows * 128u);
@@ -126,15 +134,15 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   } else if (warp == 1) {
     // E2M1 operands, E8M0 scales, M = 128
     const uint32_t idesc0 = (1u << 7) | (1u << 10) | (1u << 23) | ((uint32_t)(kTM >> 4) << 24);
-    const uint32_t sf0 = pp.tmem_base + 2 * kTN;
-    Ring<kStages> ring;
+    const uint32_t sf0 = pp.tmem_base + 2 * acc_cols;
+    Ring ring(stages);
     int j = 0;
     for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
       const int buf = j & 1;
       if (j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
       fence_after_sync();
-      const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
+      const uint32_t d = pp.tmem_base + (uint32_t)(buf * acc_cols);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 15) >> 4) << 18);
       bool ok = true;
       for (int kb = 0; kb < nk; ++kb, ring.next()) {
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
         }
         fence_after_sync();
         if (elect_one()) {
-          const uint32_t base = su32(tiles + s * kStageBytes);
+          const uint32_t base = su32(tiles + s * stage_bytes);
           const uint64_t sd = rows16_desc(su32(scales + s * kScaleBytes));
           const uint64_t wd = sw128_desc(base, 16, 1024), xd = sw128_desc(base + kABytes, 16, 1024);
           const uint32_t sfa = sf0 + (uint32_t)s * kSetCols, sfb = sfa + 8;
@@ -214,11 +222,14 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     };
     bool more = advance();
     if (more) load(cur);
-    for (int q = warp - 3; more; q += kScaleWarps) {
+    Ring ring(stages);
+    for (int i = 3; i < warp; ++i) ring.next();
+    while (more) {
       kb += kScaleWarps;
       more = advance();
       if (more) load(next);
-      const int s = q % kStages, use = q / kStages;
+      const int s = ring.s;
+      const uint32_t use = ring.use;
       if (use > 0 && !pp.wait_warp(&pp.empty[s], (use - 1) & 1)) break;
       uint4 *dst = reinterpret_cast<uint4 *>(scales + s * kScaleBytes) + lane;
       const uint2(&u)[10] = cur.u;
@@ -233,18 +244,19 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       tma::fence_proxy_async_smem();  // before the tensor cores' proxy reads them
       tma::mbar_arrive(&pp.full[s]);
       cur = next;
+#pragma unroll
+      for (int i = 0; i < kScaleWarps; ++i) ring.next();
     }
   } else {
     const int ew = warp - 3 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
-    uint32_t *buf32 = reinterpret_cast<uint32_t *>(scales + kStages * kScaleBytes +
-                                                   ew * kDrainBytes);
+    uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kRingBytes + ew * kDrainBytes);
     int j = 0;
     for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
       const int m = it.m0 + quarter * 32, buf = j & 1;
       if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
       fence_after_sync();
-      drain_tile(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), true,
+      drain_tile(pp.tmem_base + (uint32_t)(buf * acc_cols) + ((uint32_t)(32 * quarter) << 16), true,
                  it.nc, grp, a.n - m, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out, buf32);
       fence_before_sync();
       __syncwarp();

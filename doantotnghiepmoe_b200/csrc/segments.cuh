@@ -14,6 +14,7 @@ struct SegTable {
   int32_t off[kMaxExperts + 1];
   int32_t tile0[kMaxExperts + 1];  // row tiles of the experts before e
   int32_t total;                   // row tiles of all experts
+  int32_t most;                    // no tile has more rows
 
   __device__ __forceinline__ int rows(int e) const { return off[e + 1] - off[e]; }
 
@@ -58,7 +59,7 @@ __device__ __forceinline__ void build_segments(SegTable &t, const int32_t *seg_o
   }
   int prev = __shfl_up_sync(0xffffffffu, top, 1);
   if (lane == 0) prev = min(max(first, 0), R);
-  int tiles = 0, off0[kPer], t0[kPer];
+  int tiles = 0, most = 0, off0[kPer], t0[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int e = lane * kPer + j;
@@ -68,6 +69,7 @@ __device__ __forceinline__ void build_segments(SegTable &t, const int32_t *seg_o
     if (e < E) {
       bad |= raw[j] != v[j];
       tiles += (v[j] - off0[j] + bn - 1) / bn;
+      most = max(most, v[j] - off0[j]);
     }
   }
   int sum = tiles;
@@ -85,7 +87,11 @@ __device__ __forceinline__ void build_segments(SegTable &t, const int32_t *seg_o
       if (e == E - 1) t.off[E] = v[j];
     }
   }
-  if (lane == 31) t.total = t.tile0[E] = sum;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) {
+    t.total = t.tile0[E] = sum;
+    t.most = min(most, bn);
+  }
   if (bad) set_status(status, kStatusBadRoute);
 }
 

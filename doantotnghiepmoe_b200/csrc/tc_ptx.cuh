@@ -117,19 +117,20 @@ __device__ __forceinline__ uint64_t rows16_desc(uint32_t saddr) {
 constexpr int kEpiWarps = 16;  // four a TMEM lane quarter
 constexpr int kThreads = 96 + 32 * kEpiWarps;
 
-// A position in a ring of S stages: the stage and the parity of its use.
-template <int S>
+// A position in a ring of `stages`: the stage, and how often the ring went round.
 struct Ring {
-  int s = 0;
-  uint32_t use = 0;  // how often the ring went round
+  int stages, s = 0;
+  uint32_t use = 0;
+  __device__ __forceinline__ explicit Ring(int n) : stages(n) {}
   __device__ __forceinline__ void next() {
-    if (++s == S) {
+    if (++s == stages) {
       s = 0;
       ++use;
     }
   }
 };
 
+// S: the most stages that a ring may have.
 template <int S>
 struct Pipe {
   uint64_t full[S], empty[S];  // stages of the shared-memory ring
@@ -153,8 +154,8 @@ struct Pipe {
   }
   // After an abort: the copies in flight land before the CTA may exit (a bounded
   // wait for the last use of each stage).
-  __device__ __forceinline__ void drain(const Ring<S> &r) {
-    for (int s = 0; s < S; ++s) {
+  __device__ __forceinline__ void drain(const Ring &r) {
+    for (int s = 0; s < r.stages; ++s) {
       const uint32_t uses = r.use + (s < r.s ? 1 : 0);
       if (uses) tma::mbar_wait(&full[s], (uses - 1) & 1, nullptr, tma::kWaitCycles / 64);
     }
