@@ -71,7 +71,7 @@ template <typename T, int KIND>
 __global__ void __launch_bounds__(kSimpleThreads) grouped_simple_kernel(GroupedArgs a) {
   __shared__ SegTable seg;
   __shared__ __align__(16) float sa[kL][kT + 4], sb[kL][kT + 4];
-  if (threadIdx.x < 32) build_segments(seg, a.seg_off, a.E, a.R, kT, a.status);
+  if (threadIdx.x < 32) build_segments(seg, a.seg_off, a.E, a.R, kT, kT, a.status);
   __syncthreads();
   const T *x = reinterpret_cast<const T *>(a.x), *w = reinterpret_cast<const T *>(a.w),
           *d = reinterpret_cast<const T *>(a.dout);
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kSimpleThreads) grouped_simple_kernel(GroupedA
                     store_as(a.out, a.out_dtype, e * a.es_w + i * a.ld_w + j, v);
                   });
     } else {
-      const int e = seg.expert_of(g, a.E);
+      const int e = seg.expert_of(g, a.E);  // tiles of kT rows
       const int i0 = (g - seg.tile0[e]) * kT;
       const int64_t r0 = seg.off[e];
       if (KIND == kGroupedFwd)

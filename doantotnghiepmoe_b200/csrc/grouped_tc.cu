@@ -57,6 +57,7 @@ constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of
 //   wgrad           p[0..3], q[0..3]: 64, 16, 4 and 1 rows
 struct Maps {
   CUtensorMap p[4], q[4];
+  FastDiv by_m, by_n;  // by the tiles of M, and of N in wgrad
 };
 constexpr size_t kSmem = 1024 + sizeof(Pipe<kMaxStages>) + sizeof(SegTable) + 16 + kRingBytes +
                          kEpiWarps * kDrainBytes;
@@ -73,29 +74,30 @@ template <int KIND>
 struct Work {
   const GroupedArgs &a;
   const SegTable &seg;
+  const Maps &maps;
   int nM, nN;
   int total;
-  __device__ __forceinline__ Work(const GroupedArgs &a_, const SegTable &s) : a(a_), seg(s) {
+  __device__ __forceinline__ Work(const GroupedArgs &a_, const SegTable &s, const Maps &m)
+      : a(a_), seg(s), maps(m) {
     nM = ((KIND == kGroupedFwd ? a.n : a.k) + kTM - 1) / kTM;
     nN = (a.n + kTN - 1) / kTN;
     total = KIND == kGroupedWgrad ? a.E * nM * nN : seg.total * nM;
   }
   __device__ __forceinline__ Item item(int w) const {
     Item it;
-    const int g = w / nM;
+    const int g = maps.by_m.div(w);
     it.m0 = (w - g * nM) * kTM;
     if (KIND == kGroupedWgrad) {
-      it.e = g / nN;
-      it.c0 = g % nN * kTN;
+      it.e = maps.by_n.div(g);
+      it.c0 = (g - it.e * nN) * kTN;
       it.nc = min(kTN, a.n - it.c0);
       it.row0 = seg.off[it.e];
       it.len = seg.rows(it.e);
     } else {
       it.e = seg.expert_of(g, a.E);
-      const int cnt = seg.rows(it.e), nt = seg.tile0[it.e + 1] - seg.tile0[it.e];
-      const int sz = tile_rows<32>(cnt, nt), t = g - seg.tile0[it.e];
-      it.c0 = seg.off[it.e] + t * sz;
-      it.nc = min(sz, cnt - t * sz);
+      const int sz = seg.size[it.e], at = (g - seg.tile0[it.e]) * sz;
+      it.c0 = seg.off[it.e] + at;
+      it.nc = min(sz, seg.rows(it.e) - at);
       it.row0 = 0;
       it.len = KIND == kGroupedFwd ? a.k : a.n;
     }
@@ -143,14 +145,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   // full: the M side's copying warp (for both), and the odd CTA's stage in the
   // even one; tempty: both CTAs drain
-  if (threadIdx.x == 0) pp.init(rank == 0 ? 2 : 1, 2 * kEpiWarps);
+  if (threadIdx.x == 0) {
+    pp.init(rank == 0 ? 2 : 1, 2 * kEpiWarps);
+    for (int i = 0; i < (kQMn ? 4 : 1); ++i) tma::prefetch_map(&maps.p[i]);
+    for (int i = 0; i < (kQMn ? 4 : 3); ++i) tma::prefetch_map(&maps.q[i]);
+  }
   if (warp == 1) tmem_alloc_pair(&pp.tmem_base, 2 * kTN);
-  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
+  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, 32, a.status);
   fence_before_sync();
   __syncthreads();
   cluster_sync();
   fence_after_sync();
-  const Work<KIND> work(a, seg);
+  const Work<KIND> work(a, seg, maps);
   // The largest tile's N side decides the stages' size and with it how many fit:
   // with the few rows of a decode batch they hold the weights alone, and more of
   // them are on their way.
@@ -347,6 +353,8 @@ cudaError_t launch_grouped_tc(GroupedKind kind, const GroupedArgs &a, cudaStream
                           fwd ? a.ld_x : a.ld_out, 64 >> i);
   }
   if (!ok) return cudaErrorInvalidValue;
+  maps.by_m = FastDiv(((kind == kGroupedFwd ? a.n : a.k) + kTM - 1) / kTM);
+  maps.by_n = FastDiv((a.n + kTN - 1) / kTN);
   if (kind == kGroupedFwd) return launch_kind<kGroupedFwd>(maps, a, s);
   if (kind == kGroupedDgrad) return launch_kind<kGroupedDgrad>(maps, a, s);
   return launch_kind<kGroupedWgrad>(maps, a, s);

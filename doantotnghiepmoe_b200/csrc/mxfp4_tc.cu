@@ -56,6 +56,7 @@ struct Scales {
 
 struct Maps {
   CUtensorMap w, x[3];  // x in boxes of 64, 32 and 16 rows
+  FastDiv by_m;         // by the tiles of M
 };
 
 __global__ void __launch_bounds__(kMxThreads, 1)
@@ -66,9 +67,13 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   SegTable &seg = *reinterpret_cast<SegTable *>(smem_raw + sizeof(P));
   uint8_t *tiles = align1024(smem_raw + sizeof(P) + sizeof(SegTable));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) pp.init(1 + 32);  // a copying warp (for both), a scale warp's lanes
+  if (threadIdx.x == 0) {
+    pp.init(1 + 32);  // a copying warp (for both), a scale warp's lanes
+    tma::prefetch_map(&maps.w);
+    for (int i = 0; i < 3; ++i) tma::prefetch_map(&maps.x[i]);
+  }
   if (warp == 1) tmem_alloc(&pp.tmem_base, kTmemCols);
-  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, a.status);
+  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, 16, a.status);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -89,13 +94,12 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   };
   const auto item = [&](int w) {
     Item it;
-    const int g = w / nM;
+    const int g = maps.by_m.div(w);
     it.m0 = (w - g * nM) * kTM;
     it.e = seg.expert_of(g, a.E);
-    const int cnt = seg.rows(it.e), nt = seg.tile0[it.e + 1] - seg.tile0[it.e];
-    const int sz = tile_rows<16>(cnt, nt), t = g - seg.tile0[it.e];
-    it.c0 = seg.off[it.e] + t * sz;
-    it.nc = min(sz, cnt - t * sz);
+    const int sz = seg.size[it.e], at = (g - seg.tile0[it.e]) * sz;
+    it.c0 = seg.off[it.e] + at;
+    it.nc = min(sz, seg.rows(it.e) - at);
     return it;
   };
 
@@ -283,6 +287,7 @@ cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
   for (int i = 0; i < 3; ++i)
     ok = ok && tc::encode_map3d(&maps.x[i], a.xc, row, (uint64_t)a.R, 1, row, row, 64 >> i);
   if (!ok) return cudaErrorInvalidValue;
+  maps.by_m = FastDiv((a.n + kTM - 1) / kTM);
   const long long items = (long long)(a.R / kTN + std::min(a.E, a.R)) * ((a.n + kTM - 1) / kTM);
   if (items > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
   mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(maps, a);

@@ -289,16 +289,6 @@ __device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int
   }
 }
 
-// Rows of the t-th of nt row tiles of an expert with cnt rows: equal tiles, a
-// multiple of kStep (the MMA's step of N), so that 300 rows become 160 + 140
-// rather than 256 + 44.  No tile is empty: nt is ceil(cnt / kMax) with kMax at
-// least 8 kStep, so cnt / nt + kStep tiles of that many rows never cover cnt
-// with nt - 1 of them, and from 8 tiles on the size is kMax.
-template <int kStep>
-__device__ __forceinline__ int tile_rows(int cnt, int nt) {
-  return ((cnt + nt - 1) / nt + kStep - 1) & ~(kStep - 1);
-}
-
 // ---- pairs of CTAs (clusters of two, cta_group::2) ---------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

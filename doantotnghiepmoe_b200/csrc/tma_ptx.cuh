@@ -79,6 +79,11 @@ __device__ __forceinline__ void load_3d(void *dst, const void *map, uint64_t *ba
       : "memory");
 }
 
+// Starts fetching a tensor map that copies will name soon.
+__device__ __forceinline__ void prefetch_map(const void *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // `bytes` (a multiple of 16) from global memory into this CTA's shared memory,
 // both 16-byte aligned; counted on bar in bytes.
 __device__ __forceinline__ void load_bulk(void *dst, const void *src, uint64_t *bar,
