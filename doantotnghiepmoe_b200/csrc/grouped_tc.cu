@@ -50,6 +50,12 @@ constexpr uint32_t kRingBytes = 6 * (kTM + kTN) / 2 * 128;
 template <int KIND>
 constexpr int kSubOf = KIND == kGroupedWgrad ? 1 : 2;
 constexpr int kMaxStages = 10;
+// The tensor cores cut each addition to a sum in TMEM off rather than round it, an
+// error that grows with the additions (1.3e-6 of the result's norm over K = 1024,
+// 4e-7 for rounded fp32 sums).  An fp32 result is therefore summed over this
+// much of K at a time, and the draining warps add the parts, rounded, in their
+// registers; results of 16 bits lose more to their own rounding.
+constexpr int kExactK = 512;
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.
@@ -165,6 +171,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       kABytes + (kQMn ? (uint32_t)(half_most + 63) / 64 * kMnBox : half_most * 128u);
   const uint32_t stage_bytes = kSub * sub_bytes;
   const int stages = min(kMaxStages, (int)(kRingBytes / stage_bytes));
+  const int part = a.out_dtype == MOE_DT_F32 ? kExactK : INT32_MAX;  // of K in one sum
 
   if (warp == 0 || warp == 2) {
     Ring ring(stages);
@@ -229,12 +236,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int w = pair; w < work.total; w += pairs) {
       const Item it = work.item(w);
       if (it.len == 0) continue;
-      const int buf = j & 1;
-      if (rank == 0 && j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
-      const uint32_t d = pp.tmem_base + (uint32_t)(buf * kTN);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 31) >> 5) << 19);
+      uint32_t d = 0;
       bool ok = true;
+      int next = 0, more = 0;  // where the next part begins; 0: the part's first MMA
       for (int k0 = 0; k0 < it.len; k0 += kSub * kTK, ring.next()) {
+        if (k0 == next) {
+          if (k0 > 0) {
+            if (rank == 0 && elect_one()) commit_pair(&pp.tfull[j & 1]);
+            ++j;
+          }
+          ok = rank != 0 || j < 2 || pp.wait_warp(&pp.tempty[j & 1], ((j >> 1) - 1) & 1);
+          if (!ok) break;
+          d = pp.tmem_base + (uint32_t)((j & 1) * kTN);
+          next = part < it.len - k0 ? k0 + part : it.len;
+          more = 0;
+        }
         if (!pp.wait_warp(&pp.full[ring.s], ring.use & 1)) {
           ok = false;
           break;
@@ -250,7 +267,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int k = 0; k < kSub * kTK / 16; ++k) {
               const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (sub_bytes >> 4);
               mma_f16_pair(d, pd0 + sub + k % (kTK / 16) * kPStep,
-                           qd0 + sub + k % (kTK / 16) * kQStep, idesc, (k0 > 0 || k > 0) ? 1u : 0u);
+                           qd0 + sub + k % (kTK / 16) * kQStep, idesc, (more || k > 0) ? 1u : 0u);
             }
           } else {
             // forward and dgrad: one block of kTK, the rest of it zeros; wgrad: the
@@ -259,15 +276,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int k = 0; k < steps; ++k) {
               const uint64_t sub = at + (uint64_t)(k / (kTK / 16)) * (sub_bytes >> 4);
               mma_f16_pair(d, pd0 + sub + k % (kTK / 16) * kPStep,
-                           qd0 + sub + k % (kTK / 16) * kQStep, idesc, (k0 > 0 || k > 0) ? 1u : 0u);
+                           qd0 + sub + k % (kTK / 16) * kQStep, idesc, (more || k > 0) ? 1u : 0u);
             }
           }
           commit_pair(&pp.empty[ring.s]);
         }
+        more = 1;
         __syncwarp();
       }
       if (!ok) break;
-      if (rank == 0 && elect_one()) commit_pair(&pp.tfull[buf]);
+      if (rank == 0 && elect_one()) commit_pair(&pp.tfull[j & 1]);
       ++j;
     }
     // no MMA still runs, and no arrival is on its way, when the pair goes on
@@ -284,21 +302,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item it = work.item(w);
       const int m = it.m0 + rank * 128 + quarter * 32;
       const int64_t at = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
-      const bool some = it.len > 0;
-      const int buf = j & 1;
-      if (some) {
-        if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
+      Sums<kTN / kTurnCols> sums;
+      if (it.len == 0) sums.zero();
+      bool ok = true;
+      for (int k0 = 0; k0 < it.len; ++j) {
+        const int buf = j & 1;
+        ok = pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1);
+        if (!ok) break;
         fence_after_sync();
-        ++j;
-      }
-      if (m < M)
-        drain_tile(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), some,
-                   it.nc, grp, M - m, a.out, a.out_dtype, at, ld, buf32);
-      if (some) {
+        if (m < M)
+          sums.take(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), it.nc,
+                    grp * 32, k0 == 0);
         fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_at(&pp.tempty[buf], 0);
+        if (lane == 0) arrive_at(&pp.tempty[buf], 0);  // the buffer is free before the stores
+        k0 = part < it.len - k0 ? k0 + part : it.len;
       }
+      if (!ok) break;
+      if (m < M) sums.store(it.nc, grp * 32, M - m, a.out, a.out_dtype, at, ld, buf32);
     }
   }
   __syncwarp();

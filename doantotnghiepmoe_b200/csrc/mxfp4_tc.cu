@@ -260,8 +260,12 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       const int m = it.m0 + quarter * 32, buf = j & 1;
       if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
       fence_after_sync();
-      drain_tile(pp.tmem_base + (uint32_t)(buf * acc_cols) + ((uint32_t)(32 * quarter) << 16), true,
-                 it.nc, grp, a.n - m, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out, buf32);
+      for (int c = grp * 32; c < it.nc; c += kTurnCols) {
+        Sums<1> sums;
+        sums.take(pp.tmem_base + (uint32_t)(buf * acc_cols) + ((uint32_t)(32 * quarter) << 16),
+                  it.nc, c, true);
+        sums.store(it.nc, c, a.n - m, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out, buf32);
+      }
       fence_before_sync();
       __syncwarp();
       if (lane == 0) tma::mbar_arrive(&pp.tempty[buf]);

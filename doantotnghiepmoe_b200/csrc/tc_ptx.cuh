@@ -91,6 +91,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -263,31 +272,61 @@ __device__ __forceinline__ void store_cols(T *out, int64_t ld, int nc, int left,
   }
 }
 
-// at: the offset of the tile's element (row 0, m0 + 32 quarter); the groups of
-// four warps take the columns in turns of 32.
-__device__ __forceinline__ void drain_tile(uint32_t trow, bool some, int nc, int grp, int left,
-                                           void *out, int out_dtype, int64_t at, int64_t ld,
-                                           uint32_t *buf) {
-  const int size = out_dtype == MOE_DT_F32 ? 4 : 2;
-  const bool vec = (((uintptr_t)out + at * size) & 15) == 0 && ((ld * size) & 15) == 0;
-  for (int c = grp * 32; c < nc; c += kEpiWarps / 4 * 32) {
-    uint32_t v[32];
-    if (some) {
-      tmem_ld32(trow + c, v);
-      tmem_wait_ld();
-    } else {
+// What a draining warp holds of a tile: the four groups of warps take its columns
+// in turns of 32, of which it holds kTurns.
+constexpr int kTurnCols = kEpiWarps / 4 * 32;
+template <int kTurns>
+struct Sums {
+  uint32_t v[kTurns][32];
+
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = 0;
-    }
-    if (out_dtype == MOE_DT_F32)
-      store_cols(reinterpret_cast<float *>(out) + at + c * ld, ld, nc - c, left, vec, buf, v);
-    else if (out_dtype == MOE_DT_BF16)
-      store_cols(reinterpret_cast<__nv_bfloat16 *>(out) + at + c * ld, ld, nc - c, left, vec, buf,
-                 v);
-    else
-      store_cols(reinterpret_cast<__half *>(out) + at + c * ld, ld, nc - c, left, vec, buf, v);
+    for (int t = 0; t < kTurns; ++t)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[t][i] = 0;
   }
-}
+  // Columns c0 .. c0 + 31 and so on out of TMEM, instead of (first) or on top of what is held.
+  __device__ __forceinline__ void take(uint32_t trow, int nc, int c0, bool first) {
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+      const int c = c0 + t * kTurnCols;
+      if (c >= nc) break;  // warp-uniform
+      if (first) {
+        tmem_ld32(trow + c, v[t]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t u[16];
+          tmem_ld16(trow + c + 16 * h, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            v[t][16 * h + i] = __float_as_uint(__uint_as_float(v[t][16 * h + i]) +
+                                               __uint_as_float(u[i]));
+        }
+      }
+    }
+    tmem_wait_ld();
+  }
+  // at: the offset of the tile's element (row 0, m0 + 32 quarter).
+  __device__ __forceinline__ void store(int nc, int c0, int left, void *out, int out_dtype,
+                                        int64_t at, int64_t ld, uint32_t *buf) const {
+    const int size = out_dtype == MOE_DT_F32 ? 4 : 2;
+    const bool vec = (((uintptr_t)out + at * size) & 15) == 0 && ((ld * size) & 15) == 0;
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+      const int c = c0 + t * kTurnCols;
+      if (c >= nc) break;  // warp-uniform
+      if (out_dtype == MOE_DT_F32)
+        store_cols(reinterpret_cast<float *>(out) + at + c * ld, ld, nc - c, left, vec, buf, v[t]);
+      else if (out_dtype == MOE_DT_BF16)
+        store_cols(reinterpret_cast<__nv_bfloat16 *>(out) + at + c * ld, ld, nc - c, left, vec,
+                   buf, v[t]);
+      else
+        store_cols(reinterpret_cast<__half *>(out) + at + c * ld, ld, nc - c, left, vec, buf, v[t]);
+    }
+  }
+};
 
 // ---- pairs of CTAs (clusters of two, cta_group::2) ---------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
