@@ -225,10 +225,10 @@ class MoeLayerEngine:
         return ld
 
     def _vec(self, name, t, n, dtype):
-        """t [n] of this type, contiguous, on this engine's device; None passes."""
-        if t is not None and (t.dtype != dtype or t.device != self._dev or t.shape != (n,) or
-                              (n > 1 and t.stride(0) != 1)):
-            self._bad(name, t, f"contiguous {dtype} [{n}]")
+        """n contiguous elements of this type on this engine's device; None passes."""
+        if t is not None and (t.dtype != dtype or t.device != self._dev or t.numel() != n or
+                              not t.is_contiguous()):
+            self._bad(name, t, f"{n} contiguous {dtype}")
 
     def _grouped(self, rows_k, rows_n, w, seg_off, result):
         import torch
@@ -290,7 +290,7 @@ class MoeLayerEngine:
         if x.dim() != 2:
             self._bad("x", x, "[T, k]")
         T, k = x.shape
-        n = T if rows is None else rows.shape[0]
+        n = T if rows is None else rows.numel()
         self._vec("rows", rows, n, torch.int32)
         self._mxfp4("MXFP4 rows of x", codes, scales, n, k)
         self._check(lib().moe_mxfp4_quantize(self._h, x.data_ptr(), _dt(x),
@@ -315,7 +315,7 @@ class MoeLayerEngine:
         import torch
         if out.dim() != 2:
             self._bad("out", out, "[R, n]")
-        (R, n), E = out.shape, seg_off.shape[0] - 1
+        (R, n), E = out.shape, seg_off.numel() - 1
         self._vec("seg_off", seg_off, E + 1, torch.int32)
         self._mxfp4("MXFP4 rows of x", xcodes, xscales, R, k)
         self._mxfp4("MXFP4 rows of w", wcodes, wscales, E * n, k)
@@ -325,29 +325,19 @@ class MoeLayerEngine:
                                                out.data_ptr(), _dt(out),
                                                self._rows("out", out, R, n), _op_stream(stream)))
 
-    def _norm_desc(self, res, blk, gains, gates, post_norm, residual_scale, eps):
-        """Shared checks: res and blk are the named [T, H] tensors of the residual
-        and of the block (None where absent); those of a kind share type and row
-        stride."""
-        import torch
-        T, H = shape = next(t for _, t in res if t is not None).shape
-        kinds = []
-        for kind in (res, blk):
-            dtype = ld = None
-            for name, t in kind:
-                if t is None:
-                    continue
-                if dtype is None:
-                    dtype, ld = t.dtype, self._rows(name, t, T, H)
-                    kinds += _dt(t), ld
-                elif t.dtype != dtype or self._rows(name, t, T, H) != ld:
-                    self._bad(name, t, f"{dtype} rows {ld} apart, as {kind[0][0]}'s,")
-        for name, t in gains:
-            self._vec(name, t, H, torch.float32)
-        for name, t in gates:
-            self._vec(name, t, T, torch.float32)
-        rd, rld, bd, bld = kinds if len(kinds) == 4 else kinds * 2
-        return MoeBlockNormDesc(T, H, rd, bd, rld, bld, post_norm, residual_scale, eps)
+    def _norm_kind(self, T, H, *named):
+        """(type, row stride) that the given [T, H] tensors share; None where there
+        are none."""
+        kind = None
+        for name, t in named:
+            if t is None:
+                continue
+            if kind is None:
+                kind = t.dtype, self._rows(name, t, T, H)
+                code = _dt(t)
+            elif t.dtype != kind[0] or self._rows(name, t, T, H) != kind[1]:
+                self._bad(name, t, f"{kind[0]} rows {kind[1]} apart")
+        return kind and (code, kind[1])
 
     def block_norm(self, x, x_out, h, w_pre=None, y=None, w_post=None, gate=None,
                    post_norm: bool = True, residual_scale: float = 1.0, eps: float = 1e-5,
@@ -356,9 +346,17 @@ class MoeLayerEngine:
         w_pre (RMS norms; post_norm=False adds gate * y).  x, x_out [T, H] of one
         type; y, h [T, H] of that type, or of any when x is f32; gains f32 [H],
         gate f32 [T]; x_out or h may be None, x_out may be x and h may be y."""
-        d = self._norm_desc((("x", x), ("x_out", x_out)), (("y", y), ("h", h)),
-                            (("w_pre", w_pre), ("w_post", w_post)), (("gate", gate),), post_norm,
-                            residual_scale, eps)
+        import torch
+        if x.dim() != 2:
+            self._bad("x", x, "[T, H]")
+        T, H = x.shape
+        f32 = torch.float32
+        self._vec("w_pre", w_pre, H, f32)
+        self._vec("w_post", w_post, H, f32)
+        self._vec("gate", gate, T, f32)
+        rd, rld = self._norm_kind(T, H, ("x", x), ("x_out", x_out))
+        bd, bld = self._norm_kind(T, H, ("y", y), ("h", h)) or (rd, rld)
+        d = MoeBlockNormDesc(T, H, rd, bd, rld, bld, post_norm, residual_scale, eps)
         self._check(lib().moe_block_norm(self._h, d, x.data_ptr(), _ptr(y), _ptr(w_post),
                                          _ptr(gate), _ptr(w_pre), _ptr(x_out), _ptr(h),
                                          _op_stream(stream)))
@@ -370,11 +368,16 @@ class MoeLayerEngine:
         given, the gradients of the gains (f32 [H]) and of the gate (f32 [T]).
         dx_out or dh may be None (zeros); dx may be dx_out and dy may be dh."""
         import torch
-        d = self._norm_desc((("x_out", x_out), ("dx_out", dx_out), ("dx", dx)),
-                            (("dh", dh), ("y", y), ("dy", dy)),
-                            (("w_pre", w_pre), ("w_post", w_post), ("dw_pre", dw_pre),
-                             ("dw_post", dw_post)), (("gate", gate), ("dgate", dgate)), post_norm,
-                            residual_scale, eps)
+        if x_out.dim() != 2:
+            self._bad("x_out", x_out, "[T, H]")
+        T, H = x_out.shape
+        for name, t, n in (("w_pre", w_pre, H), ("w_post", w_post, H), ("dw_pre", dw_pre, H),
+                           ("dw_post", dw_post, H), ("gate", gate, T), ("dgate", dgate, T)):
+            if t is not None:
+                self._vec(name, t, n, torch.float32)
+        rd, rld = self._norm_kind(T, H, ("x_out", x_out), ("dx_out", dx_out), ("dx", dx))
+        bd, bld = self._norm_kind(T, H, ("dh", dh), ("y", y), ("dy", dy)) or (rd, rld)
+        d = MoeBlockNormDesc(T, H, rd, bd, rld, bld, post_norm, residual_scale, eps)
         L = lib()
         need = L.moe_block_norm_backward_workspace(self._h, d.rows, d.hidden)
         s = _op_stream(stream) or L.moe_get_stream(self._h)
