@@ -52,10 +52,10 @@ constexpr int kSubOf = KIND == kGroupedWgrad ? 1 : 2;
 constexpr int kMaxStages = 10;
 // The tensor cores cut each addition to a sum in TMEM off rather than round it, an
 // error that grows with the additions (1.3e-6 of the result's norm over K = 1024,
-// 4e-7 for rounded fp32 sums).  An fp32 result is therefore summed over this
-// much of K at a time, and the draining warps add the parts, rounded, in their
-// registers; results of 16 bits lose more to their own rounding.
-constexpr int kExactK = 512;
+// 4e-7 for rounded fp32 sums).  An fp32 result is therefore summed over at most
+// this much of K at a time, in equal parts, and the draining warps add the parts,
+// rounded, in their registers; results of 16 bits lose more to their own rounding.
+constexpr int kExactK = 640;
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.
@@ -136,7 +136,8 @@ __device__ __forceinline__ void load_mn(uint8_t *st, const CUtensorMap (&m)[4], 
   }
 }
 
-template <int KIND>
+// PARTS: an fp32 result whose sums may be cut into parts.
+template <int KIND, bool PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ Maps maps, const GroupedArgs a) {
   constexpr bool kPMn = KIND != kGroupedFwd, kQMn = KIND == kGroupedWgrad;
@@ -171,7 +172,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       kABytes + (kQMn ? (uint32_t)(half_most + 63) / 64 * kMnBox : half_most * 128u);
   const uint32_t stage_bytes = kSub * sub_bytes;
   const int stages = min(kMaxStages, (int)(kRingBytes / stage_bytes));
-  const int part = a.out_dtype == MOE_DT_F32 ? kExactK : INT32_MAX;  // of K in one sum
+  const auto part_of = [&](int len) {  // how much of K = len goes into one sum
+    if (!PARTS || len <= kExactK) return len;
+    const int parts = (len + kExactK - 1) / kExactK;
+    return ((len + parts - 1) / parts + 127) & ~127;  // whole stages
+  };
 
   if (warp == 0 || warp == 2) {
     Ring ring(stages);
@@ -237,6 +242,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item it = work.item(w);
       if (it.len == 0) continue;
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 31) >> 5) << 19);
+      const int part = part_of(it.len);
       uint32_t d = 0;
       bool ok = true;
       int next = 0, more = 0;  // where the next part begins; 0: the part's first MMA
@@ -302,24 +308,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item it = work.item(w);
       const int m = it.m0 + rank * 128 + quarter * 32;
       const int64_t at = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
-      Sums<kTN / kTurnCols> sums;
-      if (it.len == 0) sums.zero();
-      bool ok = true;
-      for (int k0 = 0; k0 < it.len; ++j) {
-        const int buf = j & 1;
-        ok = pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1);
+      const uint32_t lanes = pp.tmem_base + ((uint32_t)(32 * quarter) << 16);
+      if constexpr (PARTS) {
+        const int part = part_of(it.len);
+        Sums<kTN / kTurnCols> sums;
+        if (it.len == 0) sums.zero();
+        bool ok = true;
+        for (int k0 = 0; k0 < it.len; k0 += part, ++j) {
+          ok = pp.wait_warp(&pp.tfull[j & 1], (j >> 1) & 1);
+          if (!ok) break;
+          fence_after_sync();
+          if (m < M) sums.take(lanes + (uint32_t)((j & 1) * kTN), it.nc, grp * 32, k0 == 0);
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) arrive_at(&pp.tempty[j & 1], 0);
+        }
         if (!ok) break;
-        fence_after_sync();
-        if (m < M)
-          sums.take(pp.tmem_base + (uint32_t)(buf * kTN) + ((uint32_t)(32 * quarter) << 16), it.nc,
-                    grp * 32, k0 == 0);
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) arrive_at(&pp.tempty[buf], 0);  // the buffer is free before the stores
-        k0 = part < it.len - k0 ? k0 + part : it.len;
+        if (m < M) sums.store(it.nc, grp * 32, M - m, a.out, a.out_dtype, at, ld, buf32);
+      } else {
+        const bool some = it.len > 0;
+        const int buf = j & 1;
+        if (some) {
+          if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
+          fence_after_sync();
+          ++j;
+        }
+        for (int c = grp * 32; c < it.nc && m < M; c += kTurnCols) {
+          Sums<1> sums;
+          if (some) sums.take(lanes + (uint32_t)(buf * kTN), it.nc, c, true);
+          else sums.zero();
+          sums.store(it.nc, c, M - m, a.out, a.out_dtype, at, ld, buf32);
+        }
+        if (some) {
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) arrive_at(&pp.tempty[buf], 0);
+        }
       }
-      if (!ok) break;
-      if (m < M) sums.store(it.nc, grp * 32, M - m, a.out, a.out_dtype, at, ld, buf32);
     }
   }
   __syncwarp();
@@ -329,18 +354,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc_pair(pp.tmem_base, 2 * kTN);
 }
 
+template <int KIND, bool PARTS>
+cudaError_t launch_as(const Maps &maps, const GroupedArgs &a, int grid, cudaStream_t s) {
+  static const cudaError_t attr = cudaFuncSetAttribute(
+      grouped_tc_kernel<KIND, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+  if (attr != cudaSuccess) return attr;
+  grouped_tc_kernel<KIND, PARTS><<<grid, kThreads, kSmem, s>>>(maps, a);
+  return cudaGetLastError();
+}
+
 template <int KIND>
 cudaError_t launch_kind(const Maps &maps, const GroupedArgs &a, cudaStream_t s) {
-  static const cudaError_t attr = cudaFuncSetAttribute(
-      grouped_tc_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-  if (attr != cudaSuccess) return attr;
   const long long nM = ((KIND == kGroupedFwd ? a.n : a.k) + kTM - 1) / kTM;
   const long long g = KIND == kGroupedWgrad ? (long long)a.E * ((a.n + kTN - 1) / kTN)
                                             : a.R / kTN + std::min(a.E, a.R);
   if (g * nM > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
   const int grid = 2 * (int)std::min<long long>(g * nM, a.sm_count / 2);
-  grouped_tc_kernel<KIND><<<grid, kThreads, kSmem, s>>>(maps, a);
-  return cudaGetLastError();
+  const int longest = KIND == kGroupedFwd ? a.k : KIND == kGroupedDgrad ? a.n : a.R;
+  return a.out_dtype == MOE_DT_F32 && longest > kExactK ? launch_as<KIND, true>(maps, a, grid, s)
+                                                        : launch_as<KIND, false>(maps, a, grid, s);
 }
 
 }  // namespace

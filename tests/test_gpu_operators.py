@@ -95,9 +95,11 @@ def test_grouped_products_without_alignment(eng, sizes, n, k):
     check_grouped(eng, SIZES[sizes], n, k, HF, F32, pad=1)
 
 
-def test_grouped_long_sums(eng):
-    """k above every staging depth, and an expert with thousands of rows."""
-    check_grouped(eng, [3, 2500, 0, 17], 48, 2056, BF, F32, pad=8)
+@pytest.mark.parametrize("n,k,out_dtype", [(48, 2056, F32), (641, 640, F32), (1300, 1281, F32),
+                                           (72, 4104, F32), (1300, 1281, BF)])
+def test_grouped_long_sums(eng, n, k, out_dtype):
+    """Sums longer than the ring and than one part, an expert with thousands of rows."""
+    check_grouped(eng, [3, 2500, 0, 17, 641], n, k, BF, out_dtype, pad=8)
 
 
 def test_grouped_normal_values(eng):
