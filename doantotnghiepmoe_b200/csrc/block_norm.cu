@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(kMaxThreads) block_norm_kernel(const BlockNorm
 
 // RING: rows through shared memory; else straight into registers.
 template <typename TX, typename TY, int V, int NE, bool RING>
-__global__ void __launch_bounds__(kBwdThreads, RING && V * NE <= 16 ? 4 : 1)
+__global__ void __launch_bounds__(V == 1 ? kMaxThreads : kBwdThreads,
+                                  V == 1 ? (NE <= 4 ? 4 : 1) : V * NE <= 16 ? 4 : 1)
     block_norm_bwd_kernel(const BlockNormArgs a, int stages) {
   __shared__ float buf[8][kMaxThreads / 32];
   __shared__ uint64_t full[kMaxRing];
@@ -365,9 +366,18 @@ __global__ void __launch_bounds__(1024) block_norm_gains_kernel(const float *par
 
 size_t type_bytes(int dt) { return dt == MOE_DT_F32 ? 4 : 2; }
 
-// Four CTAs an SM, whose rings share its 227 KB.
-constexpr int kCtasPerSm = 4;
-constexpr size_t kRingBytes = 56 * 1024;
+// The backward pass in CTAs that fill an SM's registers and whose rings share its
+// shared memory: narrow rows take small CTAs, and many.  A thread has 8 or 16
+// values of a row in pieces of 8, or, of rows without 16-byte alignment, 4 single
+// ones (8 a thread took 190 us for 6420 rows of 1001 values, 4 take 86).
+struct BwdShape {
+  int threads, per_sm;
+  size_t ring_bytes;
+  BwdShape(int H, bool vec)
+      : threads(!vec ? std::min(kMaxThreads, (H + 127) / 128 * 32) : H > 512 ? kBwdThreads : 64),
+        per_sm(H > 512 ? 4 : H > 256 ? 8 : 16),
+        ring_bytes((size_t)(224 / per_sm) * 1024) {}
+};
 
 // Threads of a row: whole warps that cover it once, 256 at most.
 int row_threads(int H, int v, int most) {
@@ -417,8 +427,7 @@ bool vec_ok(const BlockNormArgs &a) {
 }  // namespace
 
 int block_norm_backward_ctas(int rows, int H, int sm_count) {
-  (void)H;
-  return std::max(1, std::min(rows, sm_count * kCtasPerSm));
+  return std::max(1, std::min(rows, sm_count * BwdShape(H, true).per_sm));
 }
 
 cudaError_t launch_block_norm(const BlockNormArgs &a, cudaStream_t s) {
@@ -439,15 +448,17 @@ cudaError_t launch_block_norm_backward(const BlockNormArgs &a, cudaStream_t s) {
   const bool vec = vec_ok(a);
   const size_t row = (size_t)a.H * (type_bytes(a.res_dtype) * (a.dx_out ? 2 : 1) +
                                     type_bytes(a.dtype) * ((a.dh ? 1 : 0) + (a.y ? 1 : 0)));
-  const int stages = vec && a.rows > ctas ? (int)std::min<size_t>(kMaxRing, kRingBytes / row) : 0;
+  const BwdShape shape(a.H, vec);
+  const int stages =
+      vec && a.rows > ctas ? (int)std::min<size_t>(kMaxRing, shape.ring_bytes / row) : 0;
   cudaError_t e = by_types(a.res_dtype, a.dtype, [&](auto tx, auto ty) {
-    return by_width(a.H, vec, kBwdThreads, [&](auto v, auto ne) {
-      const int threads = row_threads(a.H, v(), kBwdThreads);
+    return by_width(a.H, vec, shape.threads, [&](auto v, auto ne) {
+      const int threads = row_threads(a.H, v(), shape.threads);
       if constexpr (v() == 8) {
         if (stages >= 2) {
           auto *kernel = block_norm_bwd_kernel<decltype(tx), decltype(ty), v(), ne(), true>;
           static const cudaError_t attr = cudaFuncSetAttribute(
-              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 56 * 1024);
           if (attr != cudaSuccess) return attr;
           kernel<<<ctas, threads, stages * row, s>>>(a, stages);
           return cudaGetLastError();
