@@ -400,8 +400,7 @@ cudaError_t by_width(int H, bool vec, int threads, F &&f) {
   if (ne <= 4) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
   if (ne <= 8) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
   if (ne <= 16) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-  if (ne <= 64) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
-  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 128>{});
+  return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
 }
 
 template <typename F>
@@ -457,8 +456,8 @@ cudaError_t launch_block_norm_backward(const BlockNormArgs &a, cudaStream_t s) {
       if constexpr (v() == 8) {
         if (stages >= 2) {
           auto *kernel = block_norm_bwd_kernel<decltype(tx), decltype(ty), v(), ne(), true>;
-          static const cudaError_t attr = cudaFuncSetAttribute(
-              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 56 * 1024);
+          const cudaError_t attr = cudaFuncSetAttribute(
+              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages * row));
           if (attr != cudaSuccess) return attr;
           kernel<<<ctas, threads, stages * row, s>>>(a, stages);
           return cudaGetLastError();

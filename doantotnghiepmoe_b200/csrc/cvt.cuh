@@ -44,7 +44,7 @@ struct Piece {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i)
         *reinterpret_cast<uint4 *>(w + 4 * i) =
-            c < n ? __ldg(reinterpret_cast<const uint4 *>(p + c) + i) : make_uint4(0, 0, 0, 0);
+            c < n ? reinterpret_cast<const uint4 *>(p + c)[i] : make_uint4(0, 0, 0, 0);
     } else {
       *reinterpret_cast<T *>(w) = c < n ? p[c] : T(0.0f);
     }
@@ -72,21 +72,6 @@ struct Piece {
 };
 
 // 8 consecutive elements, the pointer 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
-    const T *e = reinterpret_cast<const T *>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {

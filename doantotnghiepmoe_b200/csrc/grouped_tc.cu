@@ -356,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 template <int KIND, bool PARTS>
 cudaError_t launch_as(const Maps &maps, const GroupedArgs &a, int grid, cudaStream_t s) {
-  static const cudaError_t attr = cudaFuncSetAttribute(
+  const cudaError_t attr = cudaFuncSetAttribute(
       grouped_tc_kernel<KIND, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   if (attr != cudaSuccess) return attr;
   grouped_tc_kernel<KIND, PARTS><<<grid, kThreads, kSmem, s>>>(maps, a);

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
 
 cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
   if (a.R <= 0) return cudaSuccess;
-  static const cudaError_t attr = cudaFuncSetAttribute(
+  const cudaError_t attr = cudaFuncSetAttribute(
       mxfp4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   if (attr != cudaSuccess) return attr;
   const uint64_t row = (uint64_t)mxfp4_code_stride(a.k);

@@ -12,6 +12,7 @@ using namespace moe::host;
 namespace {
 
 constexpr int kMaxWidth = 1 << 20;
+constexpr int kMaxRows = INT32_MAX - 4096;  // a tile behind the last row has a number
 constexpr int64_t kMaxStride = (int64_t)1 << 36;  // elements: byte strides fit a tensor map
 
 template <typename... A>
@@ -40,7 +41,8 @@ moe_status launch(moe_handle *h, const char *name, void *stream, int launches, F
 moe_status check_grouped(moe_handle *h, const moe_grouped_desc *d, GroupedArgs &a) {
   if (d->num_experts < 1 || d->num_experts > kMaxExperts)
     return refuse(h, "expert count %d outside [1, %d]", d->num_experts, kMaxExperts);
-  if (d->rows < 0) return refuse(h, "negative row count %d", d->rows);
+  if (d->rows < 0 || d->rows > kMaxRows)
+    return refuse(h, "row count %d outside [0, %d]", d->rows, kMaxRows);
   if (d->n < 1 || d->n > kMaxWidth || d->k < 1 || d->k > kMaxWidth)
     return refuse(h, "widths n = %d, k = %d outside [1, %d]", d->n, d->k, kMaxWidth);
   if (!half_type(d->dtype)) return refuse(h, "operand type %d is neither F16 nor BF16", d->dtype);
@@ -197,7 +199,7 @@ extern "C" moe_status moe_grouped_mm_mxfp4(moe_handle *h, int num_experts, int r
   std::lock_guard<std::mutex> lock(h->mu);
   if (num_experts < 1 || num_experts > kMaxExperts)
     return refuse(h, "expert count %d outside [1, %d]", num_experts, kMaxExperts);
-  if (rows < 0 || n < 1 || n > kMaxWidth || k < 1 || k > kMaxWidth)
+  if (rows < 0 || rows > kMaxRows || n < 1 || n > kMaxWidth || k < 1 || k > kMaxWidth)
     return refuse(h, "rows %d, widths n = %d, k = %d", rows, n, k);
   if (!float_type(out_dtype)) return refuse(h, "type %d is none of F32, F16 and BF16", out_dtype);
   if (ld_out < n || ld_out > kMaxStride)

@@ -389,7 +389,7 @@ def test_mxfp4_product_nan_blocks(eng):
 PAIRS = [(F32, F32), (BF, BF), (HF, HF), (F32, BF), (F32, HF)]
 # (rows, width): one row, odd widths, a warp's and a block's edges, wide rows
 NORM_SHAPES = [(1, 1), (1, 2048), (3, 7), (5, 32), (2, 257), (700, 64), (9, 1000), (4, 2056),
-               (2, 5000), (2, 16384), (1300, 136), (601, 2048), (500, 4096), (450, 8192)]
+               (2, 5000), (2, 16384), (2, 16383), (1300, 136), (2500, 250), (1300, 505), (601, 2048), (602, 1001), (500, 4096), (450, 8192)]
 
 
 def norm_inputs(T, H, rd, bd, seed, gate=True):
