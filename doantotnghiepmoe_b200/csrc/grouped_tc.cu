@@ -16,17 +16,23 @@
 // for the same products, and L2 to SM traffic is what bounded that kernel (54
 // bytes a cycle and SM).  One persistent CTA an SM: two warps keep a ring of
 // stages full by TMA across items (6 blocks of 64 elements of K of both sides, or
-// more of smaller tiles), the even
-// CTA's issuing warp issues the pair's MMAs into two accumulator buffers of 256
-// TMEM columns, and 16 warps of each CTA drain one while the other fills.  The
-// odd CTA's issuing warp passes on that its stage has landed.  Tiles that reach
-// past a segment read other experts' rows and drop their columns; in wgrad,
-// where the rows are summed, the last K step's rows beyond the expert's must be
-// zeros on both sides (0 x NaN): that step's copies are cut to 16, 4 and 1 rows,
-// and the rows up to the MMA's 16 come from behind the tensor's last row, where a
-// copy reads zeros.  (Zeroing them in shared memory cost the step two fences, 2000
-// cycles in the even CTA and 11000 in the odd one while results were stored.)  Every wait on a barrier in memory is bounded, as in
+// more of smaller tiles), the even CTA's issuing warp issues the pair's MMAs into
+// two accumulator buffers of 256 TMEM columns, and 16 warps of each CTA drain one
+// while the other fills.  The odd CTA's issuing warp passes on that its stage has
+// landed.  Tiles that reach past a segment read other experts' rows and drop their
+// columns; in wgrad, where the rows are summed, the last K step's rows beyond the
+// expert's must be zeros on both sides (0 x NaN): that step's copies are cut to
+// 16, 4 and 1 rows, and the rows up to the MMA's 16 come from behind the tensor's
+// last row, where a copy reads zeros.  (Zeroing them in shared memory cost the
+// step two fences, 2000 cycles in the even CTA and 11000 in the odd one while
+// results were stored.)  Every wait on a barrier in memory is bounded, as in
 // expert_tc.cu.
+//
+// Measured on B200 (32768 rows of 128 experts, bf16): forward n = 1536, k = 2048
+// 208 us, 1.04 GB of DRAM traffic at 5.0 TB/s and 2.2 GB from L2 into the SMs, which
+// alone takes 164 us; dgrad n = 2048, k = 768 113 us (5.1 TB/s); wgrad of it 160 us,
+// of which its 403 MB of results bound the drains.  512 rows of 64 experts, n =
+// 2048, k = 1024: 50 us, 5.4 TB/s of weights.
 #include <cuda.h>
 
 #include <algorithm>

@@ -13,9 +13,14 @@
 // blocks (128 elements of K), in the order of the rows' lanes.  Scale bytes
 // lie by row in memory; four warps, each at another stage, fetch 4 of them at
 // a time and store them in the order that a 32-row copy to TMEM takes: word
-// (r % 32) * 4 + r / 32 of a 512-byte group.  192 rows of N rather than 256 leave room in TMEM for a
-// set of scales a stage beside the two buffers: a stage is filled again only
-// once its MMAs are done, and so its set is free with it.
+// (r % 32) * 4 + r / 32 of a 512-byte group.  192 rows of N rather than 256 leave
+// room in TMEM for a set of scales a stage beside the two buffers: a stage is
+// filled again only once its MMAs are done, and so its set is free with it.
+//
+// Measured on B200 (128 experts, n = 1536, k = 2048): 32768 rows 89 us, 0.32 GB of
+// DRAM traffic and 0.88 GB from L2 into the SMs, tensor pipe 29% (bound by the steps'
+// copies and waits, 780 cycles each); 64 rows 27 us, 107 MB of weights at 3.9 TB/s, of
+// which the first 4 us pass before the first stage has landed.
 #include <cuda.h>
 
 #include <algorithm>

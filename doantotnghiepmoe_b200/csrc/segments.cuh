@@ -51,6 +51,7 @@ struct FastDiv {
 // Fills the table; called by one whole warp, before a block barrier.  Lane l
 // handles experts 8 l .. 8 l + 7 and the running maximum and the tile counts
 // are joined by warp scans.  bn: the most rows of a tile.
+//
 // An expert's tiles are equal, a multiple of `step` rows (that of the MMA's N), so
 // that 300 rows in tiles of 256 at most become 160 + 140 rather than 256 + 44.
 // None is empty: with nt = ceil(rows / bn) tiles and bn at least 8 steps, nt - 1
