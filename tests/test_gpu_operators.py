@@ -702,6 +702,45 @@ def test_training_step_in_a_graph(eng):
     assert all(torch.equal(res[a], got[a]) for a in res)
 
 
+def test_two_graphs_at_once(eng):
+    """Two captured backward passes and products replayed side by side on two
+    streams: each has its own workspace, so both keep their bits."""
+    T, H, n = 700, 512, 136
+    off, _ = offsets([300, 0, 395, 5])
+    jobs = []
+    for j in range(2):
+        i = norm_inputs(T, H, F32, F32, 70 + j)
+        d = dict(i=i, x=whole((T, H), BF, 80 + j), w=whole((4, n, H), BF, 90 + j),
+                 dx=torch.empty(T, H, device="cuda"), dg=torch.empty(H, device="cuda"),
+                 out=torch.empty(T, n, device="cuda"))
+
+        def step(d=d):
+            s = torch.cuda.current_stream()
+            eng.block_norm_backward(d["i"]["x"], d["i"]["y"], d["i"]["x"], d["i"]["w_pre"],
+                                    d["dx"], d["dg"], stream=s)
+            eng.grouped_mm(d["x"], d["w"], off, d["out"], stream=s)
+
+        step()
+        d["ref"] = [d[k].clone() for k in ("dx", "dg", "out")]
+        d["graph"], d["stream"] = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(d["graph"]):
+            step()
+        jobs.append(d)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for d in jobs:
+            for k in ("dx", "dg", "out"):
+                d[k].zero_()
+        torch.cuda.synchronize()
+        for d in jobs:
+            with torch.cuda.stream(d["stream"]):
+                for _ in range(3):
+                    d["graph"].replay()
+        torch.cuda.synchronize()
+        for d in jobs:
+            assert all(torch.equal(d[k], r) for k, r in zip(("dx", "dg", "out"), d["ref"]))
+
+
 def test_two_streams_at_once(eng):
     """The same calls on two streams at the same time, without shared state."""
     streams = [torch.cuda.Stream(), torch.cuda.default_stream()]
@@ -780,6 +819,7 @@ def test_refusals(eng):
         lambda: eng.grouped_mm(x[:, :24], w, off, out),
         lambda: eng.grouped_mm(x[:9], w, off, out),
         lambda: eng.grouped_mm(x, w[0], off, out),
+        lambda: eng.grouped_mm(x, w, off.repeat_interleave(2)[::2], out),
         lambda: eng.grouped_mm(x, w.transpose(1, 2), off, out),
         lambda: eng.grouped_mm(x.t().contiguous().t(), w, off, out),
         lambda: eng.grouped_mm(x[:1].expand(10, 32), w, off, out),
