@@ -23,6 +23,7 @@
 // (a power of two) where rows are few.  196608 x 2048 bf16 values on B200: 158 us to
 // quantise (6.4 TB/s), 182 us back (5.6 TB/s).
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "../../include/moe_b200.h"
@@ -114,6 +115,7 @@ struct SpanWalk {
     part = (int)(w & (parts - 1));
     row = w >> shift;
     step = ((long long)gridDim.x * (kQThreads / 32)) >> shift;
+    if (row >= step) row = LLONG_MAX / 2;  // a part of a row's warps only: no work
   }
 };
 

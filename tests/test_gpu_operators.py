@@ -242,7 +242,7 @@ def mx_bytes(nib):
 
 
 @pytest.mark.parametrize("R,k", [(1, 1), (3, 31), (2, 32), (5, 33), (7, 100), (1, 256), (4, 1000),
-                                 (33, 2048), (2, 4104)])
+                                 (33, 2048), (2, 4104), (5, 20000), (700, 9000)])
 @pytest.mark.parametrize("dtype", [F32, BF, HF])
 def test_mxfp4_quantize_and_back(eng, R, k, dtype):
     g = torch.Generator().manual_seed(R * 1000 + k)
