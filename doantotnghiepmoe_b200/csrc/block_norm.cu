@@ -371,13 +371,14 @@ size_t type_bytes(int dt) { return dt == MOE_DT_F32 ? 4 : 2; }
 // shared memory: narrow rows take small CTAs, and many.  A thread has 8 or 16
 // values of a row in pieces of 8, or, of rows without 16-byte alignment, 4 single
 // ones (8 a thread took 190 us for 6420 rows of 1001 values, 4 take 86).
+constexpr size_t kMaxRingBytes = 56 * 1024;  // of a CTA: a quarter of an SM's 224 KB
 struct BwdShape {
   int threads, per_sm;
   size_t ring_bytes;
   BwdShape(int H, bool vec)
       : threads(!vec ? std::min(kMaxThreads, (H + 127) / 128 * 32) : H > 512 ? kBwdThreads : 64),
         per_sm(H > 512 ? 4 : H > 256 ? 8 : 16),
-        ring_bytes((size_t)(224 / per_sm) * 1024) {}
+        ring_bytes(kMaxRingBytes * 4 / per_sm) {}
 };
 
 // Threads of a row: whole warps that cover it once, 256 at most.
@@ -457,8 +458,11 @@ cudaError_t launch_block_norm_backward(const BlockNormArgs &a, cudaStream_t s) {
       if constexpr (v() == 8) {
         if (stages >= 2) {
           auto *kernel = block_norm_bwd_kernel<decltype(tx), decltype(ty), v(), ne(), true>;
+          // One bound for every width: the attribute belongs to the kernel, which all
+          // handles and host threads of the process launch, and a smaller one set
+          // between another call's own and its launch would refuse that launch.
           const cudaError_t attr = cudaFuncSetAttribute(
-              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages * row));
+              kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxRingBytes);
           if (attr != cudaSuccess) return attr;
           kernel<<<ctas, threads, stages * row, s>>>(a, stages);
           return cudaGetLastError();

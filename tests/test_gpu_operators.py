@@ -2,6 +2,8 @@
 forms.  Whole-number inputs whose sums fit fp32 make the products exact, so
 most of them are compared bit for bit; the rest is held to bounds counted in
 roundings (half a step of the result's type, u = 2^-24 for an fp32 one)."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -582,6 +584,75 @@ def test_block_norm_gradient_by_differences(eng):
     terms = [(a.double() * dirs[k]).sum() for a, k in
              ((dx, "x"), (dy, "y"), (dwq, "w_pre"), (dwp, "w_post"), (dg, "gate"))]
     assert abs(float(sum(terms) - diff)) <= 1e-3 * float(sum(t.abs() for t in terms))
+
+
+@pytest.mark.parametrize("dt,widths", [(F32, (1152, 1536)), (BF, (2048, 1032))])
+def test_block_norm_backward_from_two_threads(eng, dt, widths):
+    """Two engines on two host threads, each with its own width and stream: the
+    widths run the same kernel with rings of different sizes, and no call is
+    refused.  The calls go straight to the C ABI, which two threads are inside of
+    at the same time then (the interpreter's lock is free only there)."""
+    T, L, jobs = 600, M.lib(), []
+    for j, H in enumerate(widths):
+        i = norm_inputs(T, H, dt, dt, 100 + H)
+        g = torch.Generator("cuda").manual_seed(H)
+        dxo, dh = (torch.randn(T, H, device="cuda", generator=g).to(dt) for _ in range(2))
+        e, stream = M.MoeLayerEngine(M.MoeConfig(64, 32, 8, 2, True, 16, 1)), torch.cuda.Stream()
+        got, ref = ([torch.empty_like(dxo), torch.empty_like(dh)] for _ in range(2))
+        eng.block_norm_backward(dxo, dh, i["x"], i["w_pre"], ref[0], y=i["y"],
+                                w_post=i["w_post"], gate=i["gate"], dy=ref[1])
+        need = L.moe_block_norm_backward_workspace(e._h, T, H)
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        code = {F32: _lib.MOE_DT_F32, BF: _lib.MOE_DT_BF16}[dt]
+        d = _lib.MoeBlockNormDesc(T, H, code, code, H, H, 1, 1.0, 1e-5)
+        args = (e._h, d, *(t.data_ptr() for t in (dxo, dh, i["x"], i["y"], i["w_post"], i["gate"],
+                                                  i["w_pre"], *got)),
+                None, None, None, ws.data_ptr(), need, stream.cuda_stream)
+        jobs.append(dict(args=args, e=e, got=got, ref=ref, stream=stream, keep=(i, dxo, dh, ws),
+                         refused=0))
+    torch.cuda.synchronize()
+    start = threading.Barrier(2)
+
+    def work(job):
+        f, args = L.moe_block_norm_backward, job["args"]
+        start.wait(60)
+        for n in range(10000):
+            job["refused"] += f(*args) != _lib.MOE_OK
+            if n % 500 == 499:
+                job["stream"].synchronize()
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    errors = [(j["refused"], L.moe_last_error(j["e"]._h)) for j in jobs]
+    for j in jobs:
+        j["e"].close()
+    assert [n for n, _ in errors] == [0, 0], errors
+    for j in jobs:
+        assert all(map(torch.equal, j["got"], j["ref"]))
+
+
+@pytest.mark.parametrize("dt,widths", [(F32, (1152, 1536)), (BF, (2048, 1032))])
+def test_block_norm_backward_widths_in_one_graph(eng, dt, widths):
+    """One graph with both widths, the larger ring captured first."""
+    jobs = []
+    for H in widths:
+        i = norm_inputs(600, H, dt, dt, 200 + H)
+        dx, ref = torch.empty_like(i["x"]), torch.empty_like(i["x"])
+        eng.block_norm_backward(i["x"], i["y"], i["x"], i["w_pre"], ref)
+        jobs.append((i, dx, ref))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i, dx, _ in jobs:
+            eng.block_norm_backward(i["x"], i["y"], i["x"], i["w_pre"], dx,
+                                    stream=torch.cuda.current_stream())
+    graph.replay()
+    torch.cuda.synchronize()
+    for _, dx, ref in jobs:
+        assert torch.equal(dx, ref)
 
 
 # --------------------------------------------------------------------------
