@@ -8,8 +8,8 @@
 // Backward, with c = dh w_pre, rq = 1 / rms(x'), rp = 1 / rms(y):
 //   D  = dx' + rq c - x' rq^3 <c, x'> / H
 //   dx = a D         dw_pre  = sum over rows of dh x' rq
-//   S  = <D w_post, y>
-//   dy = g rp (D w_post - y rp^2 S / H)      dgate = rp S
+//   t  = <D w_post, y rp>
+//   dy = g rp (D w_post - y rp t / H)        dgate = t
 //   dw_post = sum over rows of g D y rp
 // (without a post-norm dy = g D and dgate = <D, y>).
 //
@@ -17,7 +17,7 @@
 // its type.  Both passes move each value once and are bound by HBM: a row
 // stays in the registers of one CTA (8 consecutive values a thread and step)
 // from its loads to its stores, with two block sums forward (sum y^2, then
-// sum x'^2) and two backward (sum x'^2, <c, x'>, sum y^2 together, then S).
+// sum x'^2) and two backward (sum x'^2, <c, x'>, sum y^2 together, then t).
 // Forward, a CTA a row: 4096 x 2048 (fp32 residual, bf16 block) in 21 us, 4.8 TB/s
 // (a ring of rows in a few persistent CTAs took 24).  Backward, where a CTA sums
 // the gains' gradients over its rows in registers: while there are more rows than
@@ -289,8 +289,10 @@ __global__ void __launch_bounds__(V == 1 ? kMaxThreads : kBwdThreads,
     block_sums(s, buf, flip);
     const float rq = a.dh ? __frsqrt_rn(s[0] * inv_h + a.eps) : 0.0f;
     const float rp = post ? __frsqrt_rn(s[2] * inv_h + a.eps) : 1.0f;
-    const float kx = rq * rq * rq * s[1] * inv_h;
-    const float grp = (a.y && a.gate ? a.gate[r] : 1.0f) * rp;
+    // The row enters as x rq and y rp, which are of size one: rq^3 alone leaves fp32's
+    // range for rows above 1e12 or, without eps, below 1e-13, whose sums do not.
+    const float kx = rq * s[1] * inv_h * rq;
+    const float g = a.y && a.gate ? a.gate[r] : 1.0f;
     float t[1] = {0.0f}, d[NE][V];
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
@@ -302,11 +304,12 @@ __global__ void __launch_bounds__(V == 1 ? kMaxThreads : kBwdThreads,
       float o[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float xv = x[n][i], c = ch[n][i];
-        wpre[n][i] = fmaf(rq, c * xv, wpre[n][i]);
-        const float D = fmaf(-kx, xv, fmaf(rq, c * gq[n][i], dx[n][i])), Dy = D * y[n][i];
+        const float xn = rq * x[n][i], c = ch[n][i];
+        wpre[n][i] = fmaf(c, xn, wpre[n][i]);
+        const float D = fmaf(-kx, xn, fmaf(rq, c * gq[n][i], dx[n][i]));
+        const float Dy = D * (rp * y[n][i]);
         o[i] = a.scale * D;
-        wpost[n][i] = fmaf(grp, Dy, wpost[n][i]);
+        wpost[n][i] = fmaf(g, Dy, wpost[n][i]);
         t[0] = fmaf(gp[n][i], Dy, t[0]);
         d[n][i] = D * gp[n][i];
       }
@@ -314,16 +317,17 @@ __global__ void __launch_bounds__(V == 1 ? kMaxThreads : kBwdThreads,
     }
     dx_row += (int64_t)gridDim.x * a.ld_res;
     if (!a.y) continue;
+    const float grp = g * rp;
     float ky = 0.0f;
     if (post || a.dgate) {
       block_sums(t, buf, flip);
-      if (post) ky = -grp * rp * rp * t[0] * inv_h;
-      if (a.dgate && threadIdx.x == 0) a.dgate[r] = rp * t[0];
+      if (post) ky = -rp * (t[0] * inv_h);
+      if (a.dgate && threadIdx.x == 0) a.dgate[r] = t[0];
     }
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) d[n][i] = fmaf(ky, y[n][i], grp * d[n][i]);
+      for (int i = 0; i < V; ++i) d[n][i] = grp * fmaf(ky, y[n][i], d[n][i]);
       store_v<TY, V>(dy_row, (n * blockDim.x + threadIdx.x) * V, H, d[n]);
     }
     dy_row += (int64_t)gridDim.x * a.ld_blk;

@@ -557,6 +557,54 @@ def test_block_norm_backward_parts(eng):
     assert (w == 0).all()
 
 
+# The bounds of test_block_norm_backward count the roundings of the formula, whose
+# terms stay in fp32's range here: the squares reach 2^100 and 2^-100, and the
+# results differ from rows of size one by the powers of two alone.
+@pytest.mark.parametrize("T,H", [(3, 264), (3, 257), (1, 2048), (700, 1032), (2500, 64)])
+@pytest.mark.parametrize("rd,bd", [(F32, F32), (F32, BF), (BF, BF)])
+@pytest.mark.parametrize("exponent,eps", [(50, 1e-5), (-50, 0.0)])
+@pytest.mark.parametrize("post", [True, False])
+def test_block_norm_backward_of_far_rows(eng, T, H, rd, bd, exponent, eps, post):
+    """Rows of 2^50 and, without eps, of 2^-50: the terms along the row itself
+    neither vanish nor overflow."""
+    i = norm_inputs(T, H, rd, bd, 9 * T + H)
+    i["x"], i["y"] = i["x"] * 2.0 ** exponent, i["y"] * 2.0 ** exponent
+    g = torch.Generator("cuda").manual_seed(2)
+    dxo = torch.randn(T, H, device="cuda", generator=g) * 2.0 ** -exponent
+    dxo, dh = dxo.to(rd), torch.randn(T, H, device="cuda", generator=g).to(bd)
+    f = dict(device="cuda", dtype=F32)
+    got = dict(dx=torch.empty_like(i["x"]), dy=torch.empty_like(i["y"]),
+               dw_pre=torch.empty(H, **f), dw_post=torch.empty(H, **f) if post else None,
+               dgate=torch.empty(T, **f))
+    eng.block_norm_backward(dxo, dh, i["x"], i["w_pre"], got["dx"], got["dw_pre"], y=i["y"],
+                            w_post=i["w_post"], gate=i["gate"], dy=got["dy"],
+                            dw_post=got["dw_post"], dgate=got["dgate"], post_norm=post,
+                            residual_scale=0.75, eps=eps)
+    ref, mag = backward_ref(i, dxo, dh, post, 0.75, eps)
+    for k, v in got.items():
+        if v is None:
+            continue
+        steps = 256 + (T if k.startswith("dw") else 0)
+        tol = steps * U * mag[k] + half_step(v.dtype) * ref[k].abs() + torch.finfo(v.dtype).tiny
+        bad = ~((v.double() - ref[k]).abs() <= tol)
+        assert not bad.any(), (k, int(bad.sum()))
+
+
+def test_block_norm_of_far_rows(eng):
+    """The forward pass of the same rows."""
+    for exponent, eps in ((50, 1e-5), (-50, 0.0)):
+        for T, H in ((3, 264), (3, 257)):
+            i = norm_inputs(T, H, F32, F32, T + H)
+            i["x"], i["y"] = i["x"] * 2.0 ** exponent, i["y"] * 2.0 ** exponent
+            xo, h = torch.empty_like(i["x"]), torch.empty_like(i["y"])
+            eng.block_norm(i["x"], xo, h, i["w_pre"], y=i["y"], w_post=i["w_post"],
+                           gate=i["gate"], residual_scale=0.75, eps=eps)
+            rx, rh, mx, mh = norm_ref(i, True, 0.75, eps)
+            row = mx.pow(2).mean(-1, keepdim=True).sqrt() / rx.pow(2).mean(-1, keepdim=True).sqrt()
+            assert ((xo.double() - rx).abs() <= 64 * U * mx + U * rx.abs()).all()
+            assert ((h.double() - rh).abs() <= 192 * U * mh * (1 + row) + U * rh.abs()).all()
+
+
 def test_block_norm_gradient_by_differences(eng):
     """<c, x_out> + <d, h> along a direction: the central difference of the fp32
     forward pass.  With steps of 2^-8 the difference is off by its third
