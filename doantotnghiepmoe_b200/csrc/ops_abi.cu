@@ -24,6 +24,11 @@ moe_status refuse(moe_handle *h, const char *fmt, A... args) {
 size_t type_size(int dt) { return dt == MOE_DT_F32 ? 4 : 2; }
 bool half_type(int dt) { return dt == MOE_DT_F16 || dt == MOE_DT_BF16; }
 bool float_type(int dt) { return half_type(dt) || dt == MOE_DT_F32; }
+// The stride of a tensor with at most one row addresses nothing, so it neither
+// keeps a call from 16-byte accesses nor reaches a tensor map.
+int64_t row_stride(int rows, int64_t ld, int width) {
+  return rows > 1 ? ld : (int64_t)(width + 7) / 8 * 8;
+}
 bool misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
 
 template <typename F>
@@ -61,10 +66,10 @@ moe_status check_grouped(moe_handle *h, const moe_grouped_desc *d, GroupedArgs &
   a.k = d->k;
   a.dtype = d->dtype;
   a.out_dtype = d->out_dtype;
-  a.ld_x = d->ld_x;
-  a.ld_w = d->ld_w;
-  a.es_w = d->num_experts > 1 ? d->expert_stride : (int64_t)d->n * d->ld_w;
-  a.ld_out = d->ld_out;
+  a.ld_x = row_stride(d->rows, d->ld_x, d->k);
+  a.ld_w = row_stride(d->n, d->ld_w, d->k);
+  a.es_w = d->num_experts > 1 ? d->expert_stride : d->n * a.ld_w;
+  a.ld_out = row_stride(d->rows, d->ld_out, d->n);
   a.sm_count = h->sm_count;
   a.status = h->status;
   return MOE_OK;
@@ -163,8 +168,8 @@ extern "C" moe_status moe_mxfp4_quantize(moe_handle *h, const void *d_x, int dty
   if (misaligned(d_x, type_size(dtype)) || misaligned(d_index, 4) || misaligned(d_codes, 16) ||
       misaligned(d_scales, 4))
     return refuse(h, "a pointer is not aligned (codes to 16 bytes, scales to 4)");
-  Mxfp4Quant a{d_x, dtype, ld_x, d_index, src_rows, rows, k, d_codes, d_scales, h->sm_count,
-               h->status};
+  Mxfp4Quant a{d_x, dtype, row_stride(src_rows, ld_x, k), d_index, src_rows, rows, k, d_codes,
+               d_scales, h->sm_count, h->status};
   h->last_launches = 0;
   if (rows == 0) return MOE_OK;
   return launch(h, "mxfp4_quantize", stream, 1,
@@ -181,7 +186,8 @@ extern "C" moe_status moe_mxfp4_dequantize(moe_handle *h, const uint8_t *d_codes
     return refuse(h, "rows %d, width %d, row stride %lld", rows, k, (long long)ld_out);
   if (misaligned(d_out, type_size(dtype)) || misaligned(d_codes, 16) || misaligned(d_scales, 4))
     return refuse(h, "a pointer is not aligned (codes to 16 bytes, scales to 4)");
-  Mxfp4Dequant a{d_codes, d_scales, rows, k, d_out, dtype, ld_out, h->sm_count};
+  Mxfp4Dequant a{d_codes, d_scales, rows, k, d_out, dtype, row_stride(rows, ld_out, k),
+                 h->sm_count};
   h->last_launches = 0;
   if (rows == 0) return MOE_OK;
   return launch(h, "mxfp4_dequantize", stream, 1,
@@ -237,8 +243,8 @@ moe_status check_norm(moe_handle *h, const moe_block_norm_desc *d, BlockNormArgs
   a.H = d->hidden;
   a.res_dtype = d->res_dtype;
   a.dtype = d->dtype;
-  a.ld_res = d->ld_res;
-  a.ld_blk = d->ld_block;
+  a.ld_res = row_stride(d->rows, d->ld_res, d->hidden);
+  a.ld_blk = row_stride(d->rows, d->ld_block, d->hidden);
   a.post = d->post_norm != 0;
   a.scale = d->residual_scale;
   a.eps = d->eps;

@@ -212,16 +212,18 @@ class MoeLayerEngine:
 
     def _rows(self, name, t, R, width) -> int:
         """Row stride of t [R, width] on this engine's device, the elements of
-        a row side by side and its rows apart."""
+        a row side by side and its rows apart.  A single row has none: any number
+        that torch gives it stands for the same tensor, so it gets one that the
+        width alone decides and 16-byte accesses allow."""
         if t.device != self._dev or t.shape != (R, width):
             self._bad(name, t, f"[{R}, {width}]")
         ld, step = t.stride()
         if step != 1 and width > 1:
             self._bad(name, t, "rows of adjacent elements")
+        if R <= 1:
+            return (width + 7) // 8 * 8
         if ld < width:
-            if R > 1:
-                self._bad(name, t, "rows that do not overlap")
-            ld = width
+            self._bad(name, t, "rows that do not overlap")
         return ld
 
     def _vec(self, name, t, n, dtype):
@@ -246,7 +248,8 @@ class MoeLayerEngine:
         if p.dtype != q.dtype:
             raise MoeError(MOE_ERR_INVALID, f"operand types differ: {p.dtype}, {q.dtype}")
         return MoeGroupedDesc(E, R, n, k, _dt(p), _dt(result), self._rows(xname, rows_k, R, k),
-                              max(ld, k), es, self._rows(oname, rows_n, R, n))
+                              ld if n > 1 else (k + 7) // 8 * 8, es,
+                              self._rows(oname, rows_n, R, n))
 
     def grouped_mm(self, x, w, seg_off, out, stream=None):
         """out[r] = x[r] @ w[e].T for the rows r of expert e, rows sorted by

@@ -337,9 +337,9 @@ void *moe_get_stream(moe_handle *h);
  * device int32, as moe_route_permute() writes it; at most 256 experts).  Rows
  * outside every segment are neither read nor written.  Offsets that decrease
  * or leave [0, rows] are clamped and make moe_sync_status() report the fault.
- * Strides are in elements.  Base addresses and row and expert strides that are
- * multiples of 16 bytes take the tensor cores; others are computed on the SIMT
- * pipes, many times slower. */
+ * Strides are in elements; that of a tensor with a single row means nothing.
+ * Base addresses and row and expert strides that are multiples of 16 bytes take
+ * the tensor cores; others are computed on the SIMT pipes, many times slower. */
 typedef struct moe_grouped_desc {
   int32_t num_experts;
   int32_t rows;          /* R: rows of x and out; segments may cover fewer */

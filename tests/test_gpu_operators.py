@@ -703,6 +703,49 @@ def test_block_norm_backward_widths_in_one_graph(eng, dt, widths):
         assert torch.equal(dx, ref)
 
 
+def one_row(width, dtype, seed, stride=None):
+    """[1, width] with a row stride that addresses nothing."""
+    ld = stride or 3 * width + 1
+    t = torch.zeros(2, ld, device="cuda", dtype=dtype)[:1, :width]
+    t.copy_(whole((1, width), dtype, seed))
+    assert t.stride() == (ld, 1)
+    return t
+
+
+def test_one_row_has_no_stride(eng):
+    """A single row out of a wider buffer beside contiguous tensors, in every
+    call: its stride means nothing, so the results are those of a copy."""
+    H, n = 264, 136
+    x, y = one_row(H, F32, 1), one_row(H, BF, 2)
+    pre, post = torch.rand(H, device="cuda"), torch.rand(H, device="cuda")
+    res = []
+    for a, b in ((x, y), (x.contiguous().view(1, H), y.clone().view(1, H))):
+        xo, h = torch.empty(1, H, device="cuda"), torch.empty(1, H, device="cuda", dtype=BF)
+        eng.block_norm(a, xo, h, pre, y=b, w_post=post)
+        dx, dy = torch.empty(1, H, device="cuda"), one_row(H, BF, 3, stride=1001)
+        dw = torch.empty(H, device="cuda")
+        eng.block_norm_backward(a, h, xo, pre, dx, dw, y=b, w_post=post, dy=dy)
+        c = eng.mxfp4_empty(1, H)
+        eng.mxfp4_quantize(a, *c)
+        back = one_row(H, F32, 4, stride=777)
+        eng.mxfp4_dequantize(*c, back)
+        res.append([xo, h, dx, dy.clone(), dw, *c, back.clone()])
+    assert all(map(torch.equal, *res))
+    off, _ = offsets([0, 1, 0])
+    w = whole((3, n, H), BF, 5)
+    d = one_row(n, BF, 6)
+    out, dx = one_row(n, F32, 7, stride=555), one_row(H, F32, 8, stride=555)
+    dw = torch.empty(3, n, H, device="cuda")
+    eng.grouped_mm(y, w, off, out)
+    eng.grouped_mm_dgrad(d, w, off, dx)
+    eng.grouped_mm_wgrad(d, y, off, dw)
+    eng.sync_status()
+    assert torch.equal(out, (y.double() @ w[1].double().T).float())
+    assert torch.equal(dx, (d.double() @ w[1].double()).float())
+    assert torch.equal(dw[1], (d.double().T @ y.double()).float())
+    assert (dw[0] == 0).all() and (dw[2] == 0).all()
+
+
 # --------------------------------------------------------------------------
 # together, streams, graphs, refusals
 # --------------------------------------------------------------------------

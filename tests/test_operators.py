@@ -48,3 +48,26 @@ def test_host_tensors_are_refused():
         with pytest.raises(M.MoeError) as e:
             call()
         assert e.value.status == _lib.MOE_ERR_INVALID
+
+
+def test_a_single_row_has_no_stride():
+    """The stride that torch gives a one-row tensor addresses nothing: whatever it
+    is, it agrees with other tensors' and keeps 16-byte accesses."""
+    torch = pytest.importorskip("torch")
+    eng = M.MoeLayerEngine.__new__(M.MoeLayerEngine)  # no handle: only the checks run
+    eng.device, eng._dev = 0, torch.device("cpu")
+    bf = torch.bfloat16
+    wide, near = torch.zeros(4, 100)[:1, :33], torch.zeros(1, 33)
+    assert wide.stride(0) == 100 and near.stride(0) == 33
+    assert eng._norm_kind(1, 33, ("x", wide), ("x_out", near), ("none", None)) == (4, 40)
+    with pytest.raises(M.MoeError):
+        eng._norm_kind(2, 33, ("x", torch.zeros(4, 100)[:2, :33]), ("x_out", torch.zeros(2, 33)))
+    off, out = torch.zeros(3, dtype=torch.int32), torch.zeros(1, 16)
+    d = eng._grouped(torch.zeros(4, 101, dtype=bf)[:1, :24], out,
+                     torch.zeros(2, 16, 24, dtype=bf), off, out)
+    assert (d.rows, d.ld_x, d.ld_w, d.ld_out, d.expert_stride) == (1, 24, 24, 16, 384)
+    row = torch.zeros(2, 3, 32, dtype=bf)[:, :1, :24]  # experts of one row
+    out = torch.zeros(5, 1)
+    d = eng._grouped(torch.zeros(5, 24, dtype=bf), out, row.as_strided((2, 1, 24), (96, 7, 1)),
+                     off, out)
+    assert (d.n, d.ld_w, d.expert_stride, d.ld_out) == (1, 24, 96, 1)
