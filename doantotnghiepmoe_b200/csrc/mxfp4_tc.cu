@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
       for (int c = grp * 32; c < it.nc; c += kTurnCols) {
         Sums<1> sums;
         sums.take(pp.tmem_base + (uint32_t)(buf * acc_cols) + ((uint32_t)(32 * quarter) << 16),
-                  it.nc, c, true);
+                  it.nc, c);
         sums.store(it.nc, c, a.n - m, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out, buf32);
       }
       fence_before_sync();

@@ -285,28 +285,33 @@ struct Sums {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[t][i] = 0;
   }
-  // Columns c0 .. c0 + 31 and so on out of TMEM, instead of (first) or on top of what is held.
-  __device__ __forceinline__ void take(uint32_t trow, int nc, int c0, bool first) {
+  // Columns c0 .. c0 + 31 and so on out of TMEM.
+  __device__ __forceinline__ void take(uint32_t trow, int nc, int c0) {
 #pragma unroll
     for (int t = 0; t < kTurns; ++t) {
       const int c = c0 + t * kTurnCols;
       if (c >= nc) break;  // warp-uniform
-      if (first) {
-        tmem_ld32(trow + c, v[t]);
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t u[16];
-          tmem_ld16(trow + c + 16 * h, u);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            v[t][16 * h + i] = __float_as_uint(__uint_as_float(v[t][16 * h + i]) +
-                                               __uint_as_float(u[i]));
-        }
-      }
+      tmem_ld32(trow + c, v[t]);
     }
     tmem_wait_ld();
+  }
+  // The same, added to what is held.
+  __device__ __forceinline__ void add(uint32_t trow, int nc, int c0) {
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+      const int c = c0 + t * kTurnCols;
+      if (c >= nc) break;  // warp-uniform
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t u[16];
+        tmem_ld16(trow + c + 16 * h, u);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          v[t][16 * h + i] =
+              __float_as_uint(__uint_as_float(v[t][16 * h + i]) + __uint_as_float(u[i]));
+      }
+    }
   }
   // at: the offset of the tile's element (row 0, m0 + 32 quarter).
   __device__ __forceinline__ void store(int nc, int c0, int left, void *out, int out_dtype,
