@@ -56,12 +56,18 @@ constexpr uint32_t kRingBytes = 6 * (kTM + kTN) / 2 * 128;
 template <int KIND>
 constexpr int kSubOf = KIND == kGroupedWgrad ? 1 : 2;
 constexpr int kMaxStages = 10;
-// The tensor cores cut each addition to a sum in TMEM off rather than round it, an
-// error that grows with the additions (1.3e-6 of the result's norm over K = 1024,
-// 4e-7 for rounded fp32 sums).  An fp32 result is therefore summed over at most
-// this much of K at a time, in equal parts, and the draining warps add the parts,
-// rounded, in their registers; results of 16 bits lose more to their own rounding.
-constexpr int kExactK = 640;
+// The tensor cores cut each addition to a sum in TMEM off rather than round it, so the
+// error grows with the additions, 16 of K each.  Against 64 bits, normal values (in
+// brackets, of one sign), of the result's norm: one sum of K = 256 2.3e-7, 512 4.7e-7,
+// 1024 1.0e-6 (7e-7), 4096 4.4e-6 (1.0e-5), 65536 7.6e-5 (3.8e-4).  An fp32 result is
+// therefore summed over at most this much of K at a time, in equal parts, and the
+// draining warps add the parts, rounded, in their registers.  256 is the longest part
+// that loses no more than fp32 sums that round (2.5e-7 at K = 1024 for a library
+// product; parts of 128, 256 and 512 give 1.3e-7, 2.3e-7 and 4.7e-7 there, and 1.6e-7,
+// 2.4e-7, 4.8e-7 at 4096).  Its price against one sum: 512 rows of 64 experts, n =
+// 2048, k = 1024 47.2 -> 50.0 us, prefill with an fp32 result 232 -> 253 us (128: 53
+// and 275).  Results of 16 bits lose more to their own rounding.
+constexpr int kExactK = 256;
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.

@@ -123,6 +123,35 @@ def test_grouped_normal_values(eng):
             assert ((out[o[e]:o[e + 1]].double() - ref).abs() <= tol).all()
 
 
+# Each addition to a sum in tensor memory is cut off: it loses half a step on average,
+# 0.36 * 2^-23 of the sum (the mean of 1 / mantissa is 0.72), always towards zero.  Over
+# the n additions of one sum of normal products (16 of K each) that adds up to
+# 0.36 * 2^-23 n / sqrt(3) of the result's norm, as partial sums i < j have the
+# correlation sqrt(i / j).  With at most 256 of K a sum, n = 16: 4.0e-7, and adding K /
+# 256 <= 16 such sums with rounding makes it 4.1e-7 at most.  Sums of 512 of K would
+# give 8.0e-7 by that count (4.7e-7 were measured), one sum of 1024 1.6e-6 (1.0e-6).
+@pytest.mark.parametrize("K", [640, 1024, 2000, 4096])
+def test_grouped_fp32_sums_lose_no_more_than_rounded_ones(eng, K):
+    """fp32 results of normal values, forward and both gradients, the norm of the
+    error against 64 bits."""
+    g = torch.Generator("cuda").manual_seed(K)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).to(BF)
+    x, w, wt, d = r(200, K), r(2, 144, K), r(2, K, 144), r(200, K)
+    off, _ = offsets([130, 70])
+    out, dx, dw = (torch.empty(s, device="cuda") for s in ((200, 144), (200, 144), (1, 136, 144)))
+    eng.grouped_mm(x, w, off, out)
+    eng.grouped_mm_dgrad(d, wt, off, dx)
+    xr, dr = r(K, 144), r(K, 136)
+    eng.grouped_mm_wgrad(dr, xr, offsets([K])[0], dw)
+    eng.sync_status()
+    seg = [slice(0, 130), slice(130, 200)]
+    ref = [torch.cat([x[s].double() @ w[e].double().T for e, s in enumerate(seg)]),
+           torch.cat([d[s].double() @ wt[e].double() for e, s in enumerate(seg)]),
+           dr.double().T @ xr.double()]
+    for got, want in zip((out, dx, dw[0]), ref):
+        assert float((got.double() - want).norm() / want.norm()) <= 4.5e-7
+
+
 def test_grouped_nan_rows_stay_with_their_expert(eng):
     """Experts next to one with NaN and infinite rows keep exact results."""
     sizes, n, k = [21, 37, 70, 5], 72, 136
