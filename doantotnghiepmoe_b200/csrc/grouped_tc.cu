@@ -66,8 +66,14 @@ constexpr int kMaxStages = 10;
 // product; parts of 128, 256 and 512 give 1.3e-7, 2.3e-7 and 4.7e-7 there, and 1.6e-7,
 // 2.4e-7, 4.8e-7 at 4096).  Its price against one sum: 512 rows of 64 experts, n =
 // 2048, k = 1024 47.2 -> 50.0 us, prefill with an fp32 result 232 -> 253 us (128: 53
-// and 275).  Results of 16 bits lose more to their own rounding.
-constexpr int kExactK = 256;
+// and 275).  Results of 16 bits lose more to their own rounding up to the lengths
+// below: there a sum of one sign is short by 3.5e-5 of itself (fp16) and 3.8e-4 (bf16),
+// a tenth of half a step of the type.  The draining form is another kernel for each of
+// the two (Parts), so that it holds the stores of its type alone.
+enum Parts { kWhole, kPartsF32, kPartsHalf };
+__host__ __device__ constexpr int sum_limit(int out_dtype) {
+  return out_dtype == MOE_DT_F32 ? 256 : out_dtype == MOE_DT_F16 ? 8192 : 65536;
+}
 constexpr uint32_t kMnBox = kTK * 128;    // one copy of an MN-major side: 64 of M or N
 
 // Tensor maps: the M side and the N side with rows in boxes of several heights.
@@ -148,11 +154,11 @@ __device__ __forceinline__ void load_mn(uint8_t *st, const CUtensorMap (&m)[4], 
   }
 }
 
-// PARTS: an fp32 result whose sums may be cut into parts.  In wgrad the host knows
+// PARTS: the result's sums may be cut into parts.  In wgrad the host knows
 // only that an expert may have that many rows; the items of those that have fewer
 // drain as in the other form (the odd gradients of 1332 rows over 72 experts: 71.2
 // us with every item held in registers first, 68.3 so).
-template <int KIND, bool PARTS>
+template <int KIND, Parts PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_tc_kernel(const __grid_constant__ Maps maps, const GroupedArgs a) {
   constexpr bool kPMn = KIND != kGroupedFwd, kQMn = KIND == kGroupedWgrad;
@@ -188,8 +194,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t stage_bytes = kSub * sub_bytes;
   const int stages = min(kMaxStages, (int)(kRingBytes / stage_bytes));
   const auto part_of = [&](int len) {  // how much of K = len goes into one sum
-    if (!PARTS || len <= kExactK) return len;
-    const int parts = (len + kExactK - 1) / kExactK;
+    const int limit = sum_limit(PARTS == kPartsF32 ? MOE_DT_F32 : a.out_dtype);
+    if (PARTS == kWhole || len <= limit) return len;
+    const int parts = (len + limit - 1) / limit;
     return ((len + parts - 1) / parts + 127) & ~127;  // whole stages
   };
 
@@ -316,7 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {
     const int quarter = warp & 3, grp = (warp - 3) >> 2;
     uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kRingBytes + (warp - 3) * kDrainBytes);
-    const int out_dtype = PARTS ? MOE_DT_F32 : a.out_dtype;
+    const int out_dtype = PARTS == kPartsF32 ? MOE_DT_F32 : a.out_dtype;
     const int M = KIND == kGroupedFwd ? a.n : a.k;
     const int64_t ld = KIND == kGroupedFwd ? a.ld_out : KIND == kGroupedDgrad ? a.ld_x : a.ld_w;
     int j = 0;
@@ -325,7 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int m = it.m0 + rank * 128 + quarter * 32;
       const int64_t at = (KIND == kGroupedWgrad ? it.e * a.es_w : 0) + it.c0 * ld + m;
       const uint32_t lanes = pp.tmem_base + ((uint32_t)(32 * quarter) << 16);
-      if (PARTS && part_of(it.len) < it.len) {
+      if (PARTS != kWhole && part_of(it.len) < it.len) {
         const int part = part_of(it.len);
         Sums<kTN / kTurnCols> sums;
         sums.zero();
@@ -370,7 +377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc_pair(pp.tmem_base, 2 * kTN);
 }
 
-template <int KIND, bool PARTS>
+template <int KIND, Parts PARTS>
 cudaError_t launch_as(const Maps &maps, const GroupedArgs &a, int grid, cudaStream_t s) {
   const cudaError_t attr = cudaFuncSetAttribute(
       grouped_tc_kernel<KIND, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
@@ -387,8 +394,9 @@ cudaError_t launch_kind(const Maps &maps, const GroupedArgs &a, cudaStream_t s) 
   if (g * nM > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
   const int grid = 2 * (int)std::min<long long>(g * nM, a.sm_count / 2);
   const int longest = KIND == kGroupedFwd ? a.k : KIND == kGroupedDgrad ? a.n : a.R;
-  return a.out_dtype == MOE_DT_F32 && longest > kExactK ? launch_as<KIND, true>(maps, a, grid, s)
-                                                        : launch_as<KIND, false>(maps, a, grid, s);
+  if (longest <= sum_limit(a.out_dtype)) return launch_as<KIND, kWhole>(maps, a, grid, s);
+  return a.out_dtype == MOE_DT_F32 ? launch_as<KIND, kPartsF32>(maps, a, grid, s)
+                                   : launch_as<KIND, kPartsHalf>(maps, a, grid, s);
 }
 
 }  // namespace

@@ -152,6 +152,37 @@ def test_grouped_fp32_sums_lose_no_more_than_rounded_ones(eng, K):
         assert float((got.double() - want).norm() / want.norm()) <= 4.5e-7
 
 
+# A part of a 16-bit result's sum takes at most 512 additions (8192 of K, fp16) or 4096
+# (65536, bf16).  Each loses less than a step, 2^-23 of the partial sum, whose mean over
+# a same-signed sum is half of the result: 2^-15 and 2^-12 at most, a sixteenth of the
+# result type's half step.  The parts' rounded additions (at most 64) and the result's
+# own rounding to fp32 are below another sixteenth.
+@pytest.mark.parametrize("dtype,K", [(HF, 2 ** 18), (BF, 2 ** 20), (HF, 20000), (HF, 8192),
+                                     (BF, 100001)])
+def test_grouped_16_bit_sums_of_one_sign(eng, dtype, K):
+    """16-bit results over many values of one sign: forward, dgrad and the weight
+    gradient of an expert with that many rows (and of one with few)."""
+    g = torch.Generator("cuda").manual_seed(K)
+    r = lambda *s: (1 + torch.rand(*s, device="cuda", generator=g))
+    pad = -(-K // 8) * 8
+    x = r(5, pad).to(dtype)[:, :K]
+    w = (r(1, 16, pad) / 32).to(dtype)[:, :, :K]
+    out = torch.empty(5, 16, device="cuda", dtype=dtype)
+    eng.grouped_mm(x, w, offsets([5])[0], out)
+    wt = (r(1, K, 16) / 32).to(dtype)
+    dx = torch.empty(5, 16, device="cuda", dtype=dtype)
+    eng.grouped_mm_dgrad(x, wt, offsets([5])[0], dx)
+    xr, dr = r(K + 9, 16).to(dtype), (r(K + 9, 8) / 32).to(dtype)
+    dw = torch.empty(3, 8, 16, device="cuda", dtype=dtype)
+    eng.grouped_mm_wgrad(dr, xr, offsets([9, 0, K])[0], dw)
+    eng.sync_status()
+    for got, ref in ((out, x.double() @ w[0].double().T), (dx, x.double() @ wt[0].double()),
+                     (dw[0], dr[:9].double().T @ xr[:9].double()),
+                     (dw[2], dr[9:].double().T @ xr[9:].double())):
+        assert ((got.double() - ref).abs() <= 1.125 * half_step(dtype) * ref.abs()).all()
+    assert (dw[1] == 0).all()
+
+
 def test_grouped_nan_rows_stay_with_their_expert(eng):
     """Experts next to one with NaN and infinite rows keep exact results."""
     sizes, n, k = [21, 37, 70, 5], 72, 136
