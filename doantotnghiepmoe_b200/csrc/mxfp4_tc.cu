@@ -35,7 +35,21 @@ namespace {
 
 using namespace tcp;
 
-constexpr int kTM = 128, kTN = 192;
+constexpr int kTM = 128;
+// Rows of x in a tile.  A draining warp that adds parts (below) holds 32 columns for
+// each 128 of them, and its registers have room for one such turn.
+constexpr int tile_rows(bool parts) { return parts ? 128 : 192; }
+constexpr int kTN = tile_rows(false);
+// An addition to a sum in TMEM takes 64 of K and is cut off rather than rounded.
+// Against 64 bits, values of blocks with different scales, of the result's norm: one
+// sum of K = 1024 1.6e-7, 2048 2.9e-7, 4096 5.6e-7, 16384 2.5e-6, 262144 5.4e-5 (7.8e-5
+// of one sign).  So an fp32 result is summed over at most 2048 of K at a time, where
+// fp32 sums that round lose as much (2.9e-7 for a library product of the decoded
+// values), and an fp16 one over 2^17, a tenth of half its step; bf16 loses less than
+// that over every width.  In steps of 256 of K:
+__host__ __device__ constexpr int sum_limit(int out_dtype) {
+  return out_dtype == MOE_DT_F32 ? 8 : out_dtype == MOE_DT_F16 ? 512 : 4096;
+}
 constexpr uint32_t kABytes = kTM * 128;
 constexpr int kMaxStages = 8;
 constexpr int kGroup = 512;            // scale bytes of 128 rows and 4 blocks
@@ -64,6 +78,8 @@ struct Maps {
   FastDiv by_m;         // by the tiles of M
 };
 
+// PARTS: K is longer than one sum may be.
+template <bool PARTS>
 __global__ void __launch_bounds__(kMxThreads, 1)
     mxfp4_tc_kernel(const __grid_constant__ Maps maps, const Mxfp4Args a) {
   extern __shared__ uint8_t smem_raw[];
@@ -78,7 +94,7 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     for (int i = 0; i < 3; ++i) tma::prefetch_map(&maps.x[i]);
   }
   if (warp == 1) tmem_alloc(&pp.tmem_base, kTmemCols);
-  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, kTN, 16, a.status);
+  if (warp == 3) build_segments(seg, a.seg_off, a.E, a.R, tile_rows(PARTS), 16, a.status);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -93,6 +109,11 @@ __global__ void __launch_bounds__(kMxThreads, 1)
                          ((int)kTmemCols - 2 * acc_cols) / kSetCols);
   uint8_t *scales = tiles + stages * stage_bytes;
   const int nM = (a.n + kTM - 1) / kTM, nk = (a.k + 255) / 256;
+  int part = nk;  // steps of one sum: equal parts
+  if (PARTS) {
+    const int limit = sum_limit(a.out_dtype), parts = (nk + limit - 1) / limit;
+    part = (nk + parts - 1) / parts;
+  }
   const int total = seg.total * nM;
   struct Item {
     int e, m0, c0, nc;
@@ -148,14 +169,23 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     int j = 0;
     for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
       const Item it = item(w);
-      const int buf = j & 1;
-      if (j >= 2 && !pp.wait_warp(&pp.tempty[buf], ((j >> 1) - 1) & 1)) break;
+      if (j >= 2 && !pp.wait_warp(&pp.tempty[j & 1], ((j >> 1) - 1) & 1)) break;
       fence_after_sync();
-      const uint32_t d = pp.tmem_base + (uint32_t)(buf * acc_cols);
+      uint32_t d = pp.tmem_base + (uint32_t)((j & 1) * acc_cols);
       const uint32_t idesc = idesc0 | ((uint32_t)((it.nc + 15) >> 4) << 18);
       bool ok = true;
+      int first = 0;  // step that opens the running sum
       for (int kb = 0; kb < nk; ++kb, ring.next()) {
         const int s = ring.s;
+        if (PARTS && kb == first + part) {  // the next part, in the other buffer
+          if (elect_one()) commit(&pp.tfull[j & 1]);
+          ++j;
+          ok = j < 2 || pp.wait_warp(&pp.tempty[j & 1], ((j >> 1) - 1) & 1);
+          if (!ok) break;
+          fence_after_sync();
+          d = pp.tmem_base + (uint32_t)((j & 1) * acc_cols);
+          first = kb;
+        }
         if (!pp.wait_warp(&pp.full[s], ring.use & 1)) {
           ok = false;
           break;
@@ -176,14 +206,14 @@ __global__ void __launch_bounds__(kMxThreads, 1)
           for (int k = 0; k < 4; ++k) {
             const uint32_t id = (uint32_t)(k & 1) * 2;  // bytes 0-1 or 2-3 of a scale word
             mma_mxf4(d, wd + 2 * k, xd + 2 * k, idesc | (id << 4) | (id << 29), sfa + 4 * (k >> 1),
-                     sfb + 8 * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
+                     sfb + 8 * (k >> 1), (kb > first || k > 0) ? 1u : 0u);
           }
           commit(&pp.empty[s]);
         }
         __syncwarp();
       }
       if (!ok) break;
-      if (elect_one()) commit(&pp.tfull[buf]);
+      if (elect_one()) commit(&pp.tfull[j & 1]);
     }
     if (elect_one()) commit(&pp.done);
   } else if (warp < 3 + kScaleWarps) {
@@ -260,20 +290,40 @@ __global__ void __launch_bounds__(kMxThreads, 1)
     const int ew = warp - 3 - kScaleWarps, quarter = warp & 3, grp = ew >> 2;
     uint32_t *buf32 = reinterpret_cast<uint32_t *>(tiles + kRingBytes + ew * kDrainBytes);
     int j = 0;
-    for (int w = blockIdx.x; w < total; w += gridDim.x, ++j) {
+    for (int w = blockIdx.x; w < total; w += gridDim.x) {
       const Item it = item(w);
-      const int m = it.m0 + quarter * 32, buf = j & 1;
-      if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
-      fence_after_sync();
-      for (int c = grp * 32; c < it.nc; c += kTurnCols) {
+      const int m = it.m0 + quarter * 32;
+      const int64_t at = it.c0 * a.ld_out + m;
+      const uint32_t lanes = pp.tmem_base + ((uint32_t)(32 * quarter) << 16);
+      if constexpr (PARTS) {
         Sums<1> sums;
-        sums.take(pp.tmem_base + (uint32_t)(buf * acc_cols) + ((uint32_t)(32 * quarter) << 16),
-                  it.nc, c);
-        sums.store(it.nc, c, a.n - m, a.out, a.out_dtype, it.c0 * a.ld_out + m, a.ld_out, buf32);
+        sums.zero();
+        bool ok = true;
+        for (int kb = 0; kb < nk; kb += part, ++j) {
+          ok = pp.wait_warp(&pp.tfull[j & 1], (j >> 1) & 1);
+          if (!ok) break;
+          fence_after_sync();
+          sums.add(lanes + (uint32_t)((j & 1) * acc_cols), it.nc, grp * 32);
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tma::mbar_arrive(&pp.tempty[j & 1]);
+        }
+        if (!ok) break;
+        sums.store(it.nc, grp * 32, a.n - m, a.out, a.out_dtype, at, a.ld_out, buf32);
+      } else {
+        const int buf = j & 1;
+        if (!pp.wait_warp(&pp.tfull[buf], (j >> 1) & 1)) break;
+        ++j;
+        fence_after_sync();
+        for (int c = grp * 32; c < it.nc; c += kTurnCols) {
+          Sums<1> sums;
+          sums.take(lanes + (uint32_t)(buf * acc_cols), it.nc, c);
+          sums.store(it.nc, c, a.n - m, a.out, a.out_dtype, at, a.ld_out, buf32);
+        }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tma::mbar_arrive(&pp.tempty[buf]);
       }
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tma::mbar_arrive(&pp.tempty[buf]);
     }
   }
   if (threadIdx.x == 32) tma::mbar_wait(&pp.done, 0, nullptr);  // no MMA still runs
@@ -283,13 +333,23 @@ __global__ void __launch_bounds__(kMxThreads, 1)
   if (warp == 1) tmem_dealloc(pp.tmem_base, kTmemCols);
 }
 
+template <bool PARTS>
+cudaError_t launch_as(const Maps &maps, const Mxfp4Args &a, cudaStream_t s) {
+  const cudaError_t attr = cudaFuncSetAttribute(
+      mxfp4_tc_kernel<PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+  if (attr != cudaSuccess) return attr;
+  const long long items = (long long)(a.R / tile_rows(PARTS) + std::min(a.E, a.R)) *
+                          ((a.n + kTM - 1) / kTM);
+  if (items > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
+  mxfp4_tc_kernel<PARTS><<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(
+      maps, a);
+  return cudaGetLastError();
+}
+
 }  // namespace
 
 cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
   if (a.R <= 0) return cudaSuccess;
-  const cudaError_t attr = cudaFuncSetAttribute(
-      mxfp4_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-  if (attr != cudaSuccess) return attr;
   const uint64_t row = (uint64_t)mxfp4_code_stride(a.k);
   Maps maps;
   bool ok = tc::encode_map3d(&maps.w, a.wc, row, (uint64_t)a.n, (uint64_t)a.E, row, row * a.n, kTM);
@@ -297,10 +357,8 @@ cudaError_t launch_mxfp4_mm(const Mxfp4Args &a, cudaStream_t s) {
     ok = ok && tc::encode_map3d(&maps.x[i], a.xc, row, (uint64_t)a.R, 1, row, row, 64 >> i);
   if (!ok) return cudaErrorInvalidValue;
   maps.by_m = FastDiv((a.n + kTM - 1) / kTM);
-  const long long items = (long long)(a.R / kTN + std::min(a.E, a.R)) * ((a.n + kTM - 1) / kTM);
-  if (items > INT32_MAX / 2) return cudaErrorInvalidValue;  // item numbers are 32-bit
-  mxfp4_tc_kernel<<<(int)std::min<long long>(items, a.sm_count), kMxThreads, kSmem, s>>>(maps, a);
-  return cudaGetLastError();
+  return (a.k + 255) / 256 > sum_limit(a.out_dtype) ? launch_as<true>(maps, a, s)
+                                                    : launch_as<false>(maps, a, s);
 }
 
 }  // namespace moe

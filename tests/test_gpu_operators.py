@@ -428,6 +428,77 @@ def test_mxfp4_product_scales(eng):
         assert ((out[o[e]:o[e + 1]].double() - xe @ we.T).abs() <= tol).all()
 
 
+# One addition to a sum in tensor memory takes 64 of K here: with at most 2048 of K in a
+# sum, 0.36 * 2^-23 * 32 / sqrt(3) = 7.9e-7 of the result's norm by the count for the
+# 16-bit products above, and the rounded additions of the parts add 1e-8.  One sum of
+# all 8192 would give 3.2e-6 by that count, of 16384 6.3e-6 (2.5e-6 measured).
+@pytest.mark.parametrize("K", [2048, 8192, 16384, 16000])
+def test_mxfp4_fp32_sums_in_parts(eng, K):
+    """fp32 results of normal values whose blocks' scales differ, the norm of the
+    error against 64 bits."""
+    g = torch.Generator("cuda").manual_seed(K)
+    r = lambda n: (torch.randn(n, K // 32, 32, device="cuda", generator=g) * torch.exp2(
+        torch.randint(-6, 7, (n, K // 32, 1), device="cuda", generator=g).float())).view(n, K)
+    off, _ = offsets([140, 60])
+    x, w = eng.mxfp4_empty(200, K), eng.mxfp4_empty(2 * 144, K)
+    xv, wv = r(200), r(2 * 144)
+    eng.mxfp4_quantize(xv, *x)
+    eng.mxfp4_quantize(wv, *w)
+    eng.mxfp4_dequantize(*x, xv)
+    eng.mxfp4_dequantize(*w, wv)
+    out = torch.empty(200, 144, device="cuda")
+    eng.grouped_mm_mxfp4(*x, *w, off, K, out)
+    eng.sync_status()
+    xv, wv = xv.double(), wv.double().view(2, 144, K)
+    ref = torch.cat((xv[:140] @ wv[0].T, xv[140:] @ wv[1].T))
+    assert float((out.double() - ref).norm() / ref.norm()) <= 9e-7
+
+
+@pytest.mark.parametrize("sizes,n,k,out_dtype", [
+    ("ragged", 136, 4352, F32), ("tiles", 300, 2080, F32), ("tokens", 129, 10000, F32),
+    ("many", 40, 2049, F32), ("none", 32, 8192, F32), ("tokens", 8, 140000, HF)])
+def test_mxfp4_long_sums_exact(eng, sizes, n, k, out_dtype):
+    """Sums of several parts over every kind of tile.  Values are multiples of 1/4 up
+    to 12, scaled down so that 16-bit results stay finite; with signs at random the
+    sums of up to 140000 products stay below 2^24 of their grid."""
+    sizes = SIZES[sizes]
+    E = len(sizes)
+    off, R = offsets(sizes, gap=2)
+    xc, xs, xv = mx_random(R, k, 1)
+    wc, ws, wv = mx_random(E * n, k, 2, lo=123, hi=123)
+    out = torch.full((R, n), 77.0, device="cuda", dtype=out_dtype)
+    eng.grouped_mm_mxfp4(xc, xs, wc, ws, off, k, out)
+    eng.sync_status()
+    o = off.tolist()
+    for e in range(E):
+        ref = xv[o[e]:o[e + 1]] @ wv[e * n:(e + 1) * n].T
+        assert torch.equal(out[o[e]:o[e + 1]], rounded(ref, out_dtype)), e
+    assert (out[o[-1]:] == 77).all()
+
+
+# 2^20 of K in parts of 2^17: 2048 additions of one sign lose at most 2^-23 each of a
+# sum whose mean is half of the result, 2^-13, a quarter of fp16's half step.  (One sum of
+# all was 3.1e-4 short, two thirds of half a step, beside the rounding.)
+def test_mxfp4_fp16_sums_of_one_sign(eng):
+    K, n, R = 2 ** 20, 64, 40
+    g = torch.Generator("cuda").manual_seed(1)
+    c, v = [], []
+    for rows, shift in ((R, 0), (n, -24)):
+        r = 1 + torch.rand(rows, K // 32, 32, device="cuda", generator=g)
+        r *= torch.exp2(torch.randint(-6, 7, (rows, K // 32, 1), device="cuda", generator=g) +
+                        float(shift))
+        c += eng.mxfp4_empty(rows, K)
+        eng.mxfp4_quantize(r.view(rows, K), *c[-2:])
+        v.append(torch.empty(rows, K, device="cuda"))
+        eng.mxfp4_dequantize(*c[-2:], v[-1])
+    out = torch.empty(R, n, device="cuda", dtype=HF)
+    eng.grouped_mm_mxfp4(*c, offsets([R])[0], K, out)
+    eng.sync_status()
+    ref = v[0].double() @ v[1].double().T
+    assert 1 < float(ref.min()) and float(ref.max()) < 60000
+    assert ((out.double() - ref).abs() <= 1.25 * half_step(HF) * ref).all()
+
+
 def test_mxfp4_product_nan_blocks(eng):
     """A NaN block makes the outputs that use it NaN and no others."""
     sizes, n, k = [5, 6], 40, 96
