@@ -45,6 +45,7 @@
 #include "digits.cuh"
 #include "kernels.h"
 #include "route_core.cuh"
+#include "smem_bound.h"
 
 namespace moe {
 namespace {
@@ -1274,8 +1275,7 @@ cudaError_t launch_digit_decode(const DigitArgs &a_in, int sm_count, cudaStream_
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev != cached_dev || smem != cached_smem || fn != cached_fn) {
-    cudaError_t e =
-        cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem(fn, smem);
     if (e != cudaSuccess) return e;
     int per_sm = 0;
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, kDT, smem);

@@ -33,6 +33,7 @@
 #include "gemv_tiles.cuh"
 #include "kernels.h"
 #include "route_core.cuh"
+#include "smem_bound.h"
 
 namespace moe {
 namespace {
@@ -629,8 +630,7 @@ cudaError_t launch_fused_decode(const FusedArgs &a, int vec, int sm_count, uint3
   cudaGetDevice(&dev);
   if (dev != cached_dev || vec != cached_vec || smem != cached_smem ||
       (int)multi != cached_multi || a.int4 != cached_q || (int)tiles != cached_tiles) {
-    cudaError_t e =
-        cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem(fn, smem);
     if (e != cudaSuccess) return e;
     int per_sm = 0;
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, kFT, smem);

@@ -10,6 +10,7 @@
 
 #include "gemv_core.cuh"
 #include "kernels.h"
+#include "smem_bound.h"
 
 namespace moe {
 namespace {
@@ -68,8 +69,7 @@ int grid_for(int items, int sm_count) { return std::max(1, std::min(items, sm_co
 
 template <typename K>
 void ensure_smem(K kernel, size_t smem) {
-  if (smem > 48 * 1024)
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 48 * 1024) allow_smem((const void *)kernel, smem);
 }
 
 cudaError_t launch_gate_up(const GemvArgs &a, cudaStream_t s) {

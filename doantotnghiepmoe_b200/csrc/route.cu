@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "route_core.cuh"
+#include "smem_bound.h"
 
 namespace moe {
 namespace {
@@ -691,9 +692,7 @@ cudaError_t launch_route(const RouteArgs &a, cudaStream_t s, int *launches) {
       route_logits_tiled_kernel<16><<<dim3(ne, (a.T + 15) / 16), 256, 0, s>>>(a);
     }
   } else {
-    if (small_smem > 48 * 1024)
-      cudaFuncSetAttribute(route_logits_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)small_smem);
+    if (small_smem > 48 * 1024) allow_smem((const void *)route_logits_small_kernel, small_smem);
     dim3 grid((a.E + kSmallTE - 1) / kSmallTE, a.T);
     route_logits_small_kernel<<<grid, kRouteThreads, small_smem, s>>>(a);
   }
