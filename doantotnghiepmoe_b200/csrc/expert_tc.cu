@@ -39,7 +39,7 @@
 #include "common.cuh"
 #include "expert_tc.h"
 #include "digits.cuh"
-#include "tma_ptx.cuh"
+#include "tc_ptx.cuh"
 
 namespace moe {
 namespace tc {
@@ -58,31 +58,16 @@ using tma::mbar_expect_tx;
 using tma::mbar_init;
 using tma::mbar_try;
 using tma::mbar_wait;
+using tcp::fence_after_sync;
+using tcp::fence_before_sync;
+using tcp::tmem_alloc;
+using tcp::tmem_dealloc;
+using tcp::tmem_wait_ld;
 using tma::su32;
 
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar,
                                             int c0, int c1, int c2) {
   tma::load_3d(dst, map, bar, c0, c1, c2);
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t *dst_smem, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   su32(dst_smem)),
-               "r"(ncols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
-               : "memory");
-}
-
-__device__ __forceinline__ void fence_after_sync() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void fence_before_sync() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 
 __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
@@ -95,13 +80,6 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t
       : "memory");
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          su32(bar))
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int32_t v[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -110,10 +88,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int32_t v[16]) {
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
         "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_wait_ld() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // Shared-memory matrix descriptor, K-major operand with 128-byte swizzle:
@@ -203,11 +177,11 @@ __device__ __forceinline__ void mainloop(Pipe &pp, uint8_t *tiles, const CUtenso
           mma_i8(tmem + (uint32_t)(a * NB * BN), ad, bd, kIdesc, (kb > 0 || k > 0) ? 1u : 0u);
         }
       }
-      mma_commit(&pp.empty[s]);
+      tcp::commit(&pp.empty[s]);
       pp.consumed = kb + 1;
     }
     // Signals the epilogue once every issued MMA has completed.
-    mma_commit(&pp.done);
+    tcp::commit(&pp.done);
   }
 }
 
@@ -596,13 +570,13 @@ __device__ __forceinline__ void pmain(PPipe &pp, uint8_t *tiles, const CUtensorM
             mma_i8(tmem + (uint32_t)(x * NB * PBN), ad, bd, kIdesc, (kb > 0 || k > 0) ? 1u : 0u);
           }
         }
-        mma_commit(&pp.empty[s]);
+        tcp::commit(&pp.empty[s]);
         pp.consumed = q + 1;
       }
       if (!ok) break;
-      mma_commit(&pp.tfull[buf]);
+      tcp::commit(&pp.tfull[buf]);
     }
-    mma_commit(&pp.done);  // every MMA issued by this CTA has completed
+    tcp::commit(&pp.done);  // every MMA issued by this CTA has completed
   }
 }
 

@@ -1,6 +1,6 @@
-// PTX wrappers of the tensor-core instructions (tcgen05) that the grouped
-// products use, their descriptors, and the barriers of a persistent kernel
-// with two copying warps, one issuing warp and kEpiWarps draining warps.
+// PTX wrappers of the tensor-core instructions (tcgen05), and, for the grouped
+// products, their descriptors and the barriers of a persistent kernel with two
+// copying warps, one issuing warp and kEpiWarps draining warps.
 #pragma once
 
 #include <cstdint>
@@ -48,16 +48,6 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           su32(bar))
-      : "memory");
-}
-// D (+)= A B^T of f16 or bf16 operands, fp32 sums; 16 elements of K.
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // D (+)= (A sA) (B sB)^T of E2M1 operands with an E8M0 scale for 32 elements of
@@ -374,8 +364,9 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-// M = 256 over the pair: each CTA's shared memory holds its 128 rows of A and
-// its half of the rows of B, at the same places, and its TMEM 128 rows of D.
+// D (+)= A B^T of f16 or bf16 operands, fp32 sums; 16 elements of K, M = 256 over the
+// pair: each CTA's shared memory holds its 128 rows of A and its half of the rows of
+// B, at the same places, and its TMEM 128 rows of D.
 __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                              uint32_t accumulate) {
   asm volatile(

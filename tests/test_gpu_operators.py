@@ -564,6 +564,37 @@ def test_block_norm(eng, T, H, rd, bd, post, gate):
             half_step(bd) * rh.abs() + tiny[1]).all()
 
 
+@pytest.mark.parametrize("T,H", [(5, 264), (700, 1024), (2, 4096)])
+@pytest.mark.parametrize("rd,bd", [(BF, BF), (F32, HF)])
+def test_norms_off_a_16_byte_border(eng, T, H, rd, bd):
+    """Widths that 16-byte accesses would take, from addresses that they would not."""
+    i = norm_inputs(T, H, rd, bd, T + H)
+    place = lambda t: torch.cat((t.new_zeros(1), t.flatten()))[1:].view(t.shape)
+    off = {k: None if v is None else place(v) for k, v in i.items()}
+    assert off["x"].data_ptr() % 16 and off["w_pre"].data_ptr() % 16
+    xo, h = place(i["x"]), place(i["y"])
+    eng.block_norm(off["x"], xo, h, off["w_pre"], y=off["y"], w_post=off["w_post"],
+                   gate=off["gate"], residual_scale=0.75, eps=1e-5)
+    rx, rh, mx, mh = norm_ref(i, True, 0.75, 1e-5)
+    row = mx.pow(2).mean(-1, keepdim=True).sqrt() / (rx.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt()
+    tiny = torch.finfo(rd).tiny, torch.finfo(bd).tiny
+    assert ((xo.double() - rx).abs() <= 64 * U * mx + half_step(rd) * rx.abs() + tiny[0]).all()
+    assert ((h.double() - rh).abs() <= 192 * U * mh * (1 + row) +
+            half_step(bd) * rh.abs() + tiny[1]).all()
+    dxo, dh = (torch.randn(T, H, device="cuda").to(t) for t in (rd, bd))
+    got = dict(dx=place(dxo), dy=place(dh), dw_pre=place(i["w_pre"]), dw_post=place(i["w_pre"]),
+               dgate=torch.empty(T, device="cuda"))
+    eng.block_norm_backward(place(dxo), place(dh), off["x"], off["w_pre"], got["dx"],
+                            got["dw_pre"], y=off["y"], w_post=off["w_post"], gate=off["gate"],
+                            dy=got["dy"], dw_post=got["dw_post"], dgate=got["dgate"],
+                            residual_scale=0.75, eps=1e-5)
+    ref, mag = backward_ref(i, dxo, dh, True, 0.75, 1e-5)
+    for k, v in got.items():
+        steps = 256 + (T if k.startswith("dw") else 0)
+        tol = steps * U * mag[k] + half_step(v.dtype) * ref[k].abs() + torch.finfo(v.dtype).tiny
+        assert ((v.double() - ref[k]).abs() <= tol).all(), k
+
+
 def test_block_norm_parts(eng):
     """Without y (the first norm alone), without h (behind the last block),
     without gains, in place, and rows in wider buffers."""
