@@ -32,7 +32,7 @@
 // 208 us, 1.04 GB of DRAM traffic at 5.0 TB/s and 2.2 GB from L2 into the SMs, which
 // alone takes 164 us; dgrad n = 2048, k = 768 113 us (5.1 TB/s); wgrad of it 160 us,
 // of which its 403 MB of results bound the drains.  512 rows of 64 experts, n =
-// 2048, k = 1024: 50 us, 5.4 TB/s of weights.
+// 2048, k = 1024, fp32 result: 50 us, 5.4 TB/s of weights.
 #include <cuda.h>
 
 #include <algorithm>
@@ -57,19 +57,21 @@ template <int KIND>
 constexpr int kSubOf = KIND == kGroupedWgrad ? 1 : 2;
 constexpr int kMaxStages = 10;
 // The tensor cores cut each addition to a sum in TMEM off rather than round it, so the
-// error grows with the additions, 16 of K each.  Against 64 bits, normal values (in
-// brackets, of one sign), of the result's norm: one sum of K = 256 2.3e-7, 512 4.7e-7,
-// 1024 1.0e-6 (7e-7), 4096 4.4e-6 (1.0e-5), 65536 7.6e-5 (3.8e-4).  An fp32 result is
-// therefore summed over at most this much of K at a time, in equal parts, and the
-// draining warps add the parts, rounded, in their registers.  256 is the longest part
-// that loses no more than fp32 sums that round (2.5e-7 at K = 1024 for a library
-// product; parts of 128, 256 and 512 give 1.3e-7, 2.3e-7 and 4.7e-7 there, and 1.6e-7,
-// 2.4e-7, 4.8e-7 at 4096).  Its price against one sum: 512 rows of 64 experts, n =
-// 2048, k = 1024 47.2 -> 50.0 us, prefill with an fp32 result 232 -> 253 us (128: 53
-// and 275).  Results of 16 bits lose more to their own rounding up to the lengths
-// below: there a sum of one sign is short by 3.5e-5 of itself (fp16) and 3.8e-4 (bf16),
-// a tenth of half a step of the type.  The draining form is another kernel for each of
-// the two (Parts), so that it holds the stores of its type alone.
+// error grows with the additions, 16 of K each.  Against 64 bits, of the result's norm,
+// normal bf16 (fp16) values: one sum of K = 256 2.3e-7 (3.4e-7), 512 4.7e-7 (6.4e-7),
+// 1024 1.0e-6 (1.3e-6), 4096 4.4e-6 (4.9e-6), 65536 7.6e-5; values of one sign: 1024
+// 6.9e-7 (5.8e-6), 65536 3.8e-4 (4.2e-4).  A result is therefore summed over at most
+// sum_limit of K at a time, in equal parts, and the draining warps add the parts,
+// rounded, in their registers.  For an fp32 result 256 is the longest part with which
+// normal values lose no more than in fp32 sums that round, at the usual lengths (K =
+// 1024, parts of 128 / 256 / 512: 1.3e-7, 2.3e-7, 4.7e-7 in bf16, where a library
+// product has 2.5e-7; 2.0e-7, 3.4e-7, 6.5e-7 in fp16, where it has 5.7e-7; only fp16
+// values of one sign lose more, 1.1e-6 to its 4.8e-7).  Its price against one sum: 512
+// rows of 64 experts, n = 2048, k = 1024 47.2 -> 50.0 us, prefill with an fp32 result
+// 232 -> 253 us (128: 53 and 275).  Results of 16 bits lose more to their own rounding
+// up to the lengths below, where a sum of one sign is short by a tenth of half a step
+// of the type.  The draining form is another kernel for each of the two (Parts), so
+// that it holds the stores of its type alone.
 enum Parts { kWhole, kPartsF32, kPartsHalf };
 __host__ __device__ constexpr int sum_limit(int out_dtype) {
   return out_dtype == MOE_DT_F32 ? 256 : out_dtype == MOE_DT_F16 ? 8192 : 65536;

@@ -131,7 +131,7 @@ def test_grouped_normal_values(eng):
 # 256 <= 16 such sums with rounding makes it 4.1e-7 at most.  Sums of 512 of K would
 # give 8.0e-7 by that count (4.7e-7 were measured), one sum of 1024 1.6e-6 (1.0e-6).
 @pytest.mark.parametrize("K", [640, 1024, 2000, 4096])
-def test_grouped_fp32_sums_lose_no_more_than_rounded_ones(eng, K):
+def test_grouped_fp32_sums_in_parts(eng, K):
     """fp32 results of normal values, forward and both gradients, the norm of the
     error against 64 bits."""
     g = torch.Generator("cuda").manual_seed(K)
