@@ -27,7 +27,7 @@ bool float_type(int dt) { return half_type(dt) || dt == MOE_DT_F32; }
 // The stride of a tensor with at most one row addresses nothing, so it neither
 // keeps a call from 16-byte accesses nor reaches a tensor map.
 int64_t row_stride(int rows, int64_t ld, int width) {
-  return rows > 1 ? ld : (int64_t)(width + 7) / 8 * 8;
+  return rows > 1 ? ld : ((int64_t)width + 7) / 8 * 8;
 }
 bool misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
 
@@ -53,12 +53,15 @@ moe_status check_grouped(moe_handle *h, const moe_grouped_desc *d, GroupedArgs &
   if (!half_type(d->dtype)) return refuse(h, "operand type %d is neither F16 nor BF16", d->dtype);
   if (d->out_dtype != d->dtype && d->out_dtype != MOE_DT_F32)
     return refuse(h, "result type %d is neither the operands' type nor F32", d->out_dtype);
-  if (d->ld_x < d->k || d->ld_w < d->k || d->ld_out < d->n)
+  a.ld_x = row_stride(d->rows, d->ld_x, d->k);
+  a.ld_w = row_stride(d->n, d->ld_w, d->k);
+  a.ld_out = row_stride(d->rows, d->ld_out, d->n);
+  if (a.ld_x < d->k || a.ld_w < d->k || a.ld_out < d->n)
     return refuse(h, "a row stride is smaller than its row (k = %d, n = %d)", d->k, d->n);
-  if (d->ld_x > kMaxStride || d->ld_w > kMaxStride || d->ld_out > kMaxStride ||
+  if (a.ld_x > kMaxStride || a.ld_w > kMaxStride || a.ld_out > kMaxStride ||
       d->expert_stride > kMaxStride)
     return refuse(h, "a stride is above %lld elements", (long long)kMaxStride);
-  if (d->num_experts > 1 && d->expert_stride < (int64_t)(d->n - 1) * d->ld_w + d->k)
+  if (d->num_experts > 1 && d->expert_stride < (d->n - 1) * a.ld_w + d->k)
     return refuse(h, "expert stride %lld is smaller than one expert", (long long)d->expert_stride);
   a.E = d->num_experts;
   a.R = d->rows;
@@ -66,10 +69,7 @@ moe_status check_grouped(moe_handle *h, const moe_grouped_desc *d, GroupedArgs &
   a.k = d->k;
   a.dtype = d->dtype;
   a.out_dtype = d->out_dtype;
-  a.ld_x = row_stride(d->rows, d->ld_x, d->k);
-  a.ld_w = row_stride(d->n, d->ld_w, d->k);
   a.es_w = d->num_experts > 1 ? d->expert_stride : d->n * a.ld_w;
-  a.ld_out = row_stride(d->rows, d->ld_out, d->n);
   a.sm_count = h->sm_count;
   a.status = h->status;
   return MOE_OK;
@@ -160,6 +160,7 @@ extern "C" moe_status moe_mxfp4_quantize(moe_handle *h, const void *d_x, int dty
     return MOE_ERR_INVALID;
   std::lock_guard<std::mutex> lock(h->mu);
   if (!float_type(dtype)) return refuse(h, "type %d is none of F32, F16 and BF16", dtype);
+  ld_x = row_stride(src_rows, ld_x, k);
   if (rows < 0 || src_rows < 0 || k < 1 || k > kMaxWidth || ld_x < k || ld_x > kMaxStride)
     return refuse(h, "rows %d of %d, width %d, row stride %lld", rows, src_rows, k,
                   (long long)ld_x);
@@ -168,8 +169,8 @@ extern "C" moe_status moe_mxfp4_quantize(moe_handle *h, const void *d_x, int dty
   if (misaligned(d_x, type_size(dtype)) || misaligned(d_index, 4) || misaligned(d_codes, 16) ||
       misaligned(d_scales, 4))
     return refuse(h, "a pointer is not aligned (codes to 16 bytes, scales to 4)");
-  Mxfp4Quant a{d_x, dtype, row_stride(src_rows, ld_x, k), d_index, src_rows, rows, k, d_codes,
-               d_scales, h->sm_count, h->status};
+  Mxfp4Quant a{d_x, dtype, ld_x, d_index, src_rows, rows, k, d_codes, d_scales, h->sm_count,
+               h->status};
   h->last_launches = 0;
   if (rows == 0) return MOE_OK;
   return launch(h, "mxfp4_quantize", stream, 1,
@@ -182,12 +183,12 @@ extern "C" moe_status moe_mxfp4_dequantize(moe_handle *h, const uint8_t *d_codes
   if (!h || (rows > 0 && (!d_codes || !d_scales || !d_out))) return MOE_ERR_INVALID;
   std::lock_guard<std::mutex> lock(h->mu);
   if (!float_type(dtype)) return refuse(h, "type %d is none of F32, F16 and BF16", dtype);
+  ld_out = row_stride(rows, ld_out, k);
   if (rows < 0 || k < 1 || k > kMaxWidth || ld_out < k || ld_out > kMaxStride)
     return refuse(h, "rows %d, width %d, row stride %lld", rows, k, (long long)ld_out);
   if (misaligned(d_out, type_size(dtype)) || misaligned(d_codes, 16) || misaligned(d_scales, 4))
     return refuse(h, "a pointer is not aligned (codes to 16 bytes, scales to 4)");
-  Mxfp4Dequant a{d_codes, d_scales, rows, k, d_out, dtype, row_stride(rows, ld_out, k),
-                 h->sm_count};
+  Mxfp4Dequant a{d_codes, d_scales, rows, k, d_out, dtype, ld_out, h->sm_count};
   h->last_launches = 0;
   if (rows == 0) return MOE_OK;
   return launch(h, "mxfp4_dequantize", stream, 1,
@@ -208,6 +209,7 @@ extern "C" moe_status moe_grouped_mm_mxfp4(moe_handle *h, int num_experts, int r
   if (rows < 0 || rows > kMaxRows || n < 1 || n > kMaxWidth || k < 1 || k > kMaxWidth)
     return refuse(h, "rows %d, widths n = %d, k = %d", rows, n, k);
   if (!float_type(out_dtype)) return refuse(h, "type %d is none of F32, F16 and BF16", out_dtype);
+  ld_out = row_stride(rows, ld_out, n);
   if (ld_out < n || ld_out > kMaxStride)
     return refuse(h, "row stride %lld of a row of %d", (long long)ld_out, n);
   if (misaligned(d_xcodes, 16) || misaligned(d_wcodes, 16) || misaligned(d_xscales, 4) ||
@@ -234,8 +236,10 @@ moe_status check_norm(moe_handle *h, const moe_block_norm_desc *d, BlockNormArgs
       (d->res_dtype != d->dtype && d->res_dtype != MOE_DT_F32))
     return refuse(h, "residual type %d with block type %d: the same, or an F32 residual",
                   d->res_dtype, d->dtype);
-  if (d->ld_res < d->hidden || d->ld_block < d->hidden || d->ld_res > kMaxStride ||
-      d->ld_block > kMaxStride)
+  a.ld_res = row_stride(d->rows, d->ld_res, d->hidden);
+  a.ld_blk = row_stride(d->rows, d->ld_block, d->hidden);
+  if (a.ld_res < d->hidden || a.ld_blk < d->hidden || a.ld_res > kMaxStride ||
+      a.ld_blk > kMaxStride)
     return refuse(h, "row strides %lld, %lld of a row of %d", (long long)d->ld_res,
                   (long long)d->ld_block, d->hidden);
   if (!(d->eps >= 0.0f)) return refuse(h, "eps is negative or not a number");
@@ -243,8 +247,6 @@ moe_status check_norm(moe_handle *h, const moe_block_norm_desc *d, BlockNormArgs
   a.H = d->hidden;
   a.res_dtype = d->res_dtype;
   a.dtype = d->dtype;
-  a.ld_res = row_stride(d->rows, d->ld_res, d->hidden);
-  a.ld_blk = row_stride(d->rows, d->ld_block, d->hidden);
   a.post = d->post_norm != 0;
   a.scale = d->residual_scale;
   a.eps = d->eps;

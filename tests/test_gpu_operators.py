@@ -908,6 +908,35 @@ def test_one_row_has_no_stride(eng):
     assert (dw[0] == 0).all() and (dw[2] == 0).all()
 
 
+def test_one_row_with_any_stride_at_the_c_abi(eng):
+    """The stride of a single row is not looked at, 0 and huge numbers included."""
+    L, k, n = M.lib(), 72, 40
+    st = torch.cuda.current_stream().cuda_stream
+    x, w = whole((1, k), BF, 1), whole((1, n, k), BF, 2)
+    off, _ = offsets([1])
+    for ld in (0, -5, 3, 2 ** 50):
+        out, h = torch.full((n,), 7.0, device="cuda"), torch.full((k,), 7.0, device="cuda")
+        back = torch.full((k,), 7.0, device="cuda")
+        d = _lib.MoeGroupedDesc(1, 1, n, k, _lib.MOE_DT_BF16, _lib.MOE_DT_F32, ld, k, 0, ld)
+        assert L.moe_grouped_mm(eng._h, d, x.data_ptr(), w.data_ptr(), off.data_ptr(),
+                                out.data_ptr(), st) == _lib.MOE_OK
+        b = _lib.MoeBlockNormDesc(1, k, _lib.MOE_DT_F32, _lib.MOE_DT_F32, ld, ld, 1, 1.0, 1e-5)
+        xf = x.float()
+        assert L.moe_block_norm(eng._h, b, xf.data_ptr(), None, None, None, None, None,
+                                h.data_ptr(), st) == _lib.MOE_OK
+        c = eng.mxfp4_empty(1, k)
+        assert L.moe_mxfp4_quantize(eng._h, x.data_ptr(), _lib.MOE_DT_BF16, ld, 1, None, 1, k,
+                                    *(t.data_ptr() for t in c), st) == _lib.MOE_OK
+        assert L.moe_mxfp4_dequantize(eng._h, *(t.data_ptr() for t in c), 1, k, back.data_ptr(),
+                                      _lib.MOE_DT_F32, ld, st) == _lib.MOE_OK
+        eng.sync_status()
+        torch.cuda.synchronize()
+        assert torch.equal(out, (x.double() @ w[0].double().T).float()[0])
+        ref = xf[0].double() / (xf.double().pow(2).mean() + 1e-5).sqrt()
+        assert ((h.double() - ref).abs() <= 65 * U * ref.abs()).all()
+        assert torch.equal(back.cpu(), mx_ref(x)[2][0].float())
+
+
 # --------------------------------------------------------------------------
 # together, streams, graphs, refusals
 # --------------------------------------------------------------------------
